@@ -241,6 +241,93 @@ lssm_status lssm_ssd_step_batched(lssm_ctx* ctx, const void* x, const void* B, c
                                   const void* dt_bias, const void* A_log, const void* D_skip, void* state_io,
                                   void* y, lssm_ssd_batched_dims dims);
 
+/* ---- scoring: log probabilities of given tokens (no reference counterpart: the reference only
+ *      takes the argmax or a top-p sample of a step's logits, src/runtime/sampler.cpp:13-80) ----
+ * For every row of logits: lse = log sum_j e^(x_j), logp = x_t - lse of the row's target t,
+ * entropy = -sum_j p_j log p_j (p_j = e^(x_j - lse)), and the top_k largest entries as
+ * (id, x - lse), largest first, of equal ones the lower id first. Any output may be null, but not
+ * all; top_ids and top_logp (rows x top_k) go together and are given exactly when top_k > 0.
+ *   targets  one u32 per row (may be null without logp). LSSM_NO_TOKEN: logp 0; an id >= vocab: logp NaN.
+ *   -inf     (a masked entry) has p = 0 and no share of the entropy. A row of nothing but -inf has
+ *            lse = logp = top values = -inf and entropy 0.
+ *   NaN/+inf in a row makes its lse, logp, entropy and top values NaN; the ids rank NaN as -inf.
+ * logits (rows, vocab) of dtype, row_stride elements apart (0 = vocab), aligned to its element;
+ * what lies between two rows is not read. The outputs must not overlap the logits. */
+#define LSSM_NO_TOKEN 0xFFFFFFFFu
+#define LSSM_TOP_K_MAX 32u
+typedef struct {
+    uint32_t rows, vocab, top_k;
+    uint32_t dtype;        /* lssm_dtype of the logits */
+    uint64_t row_stride;
+} lssm_logprobs_dims;
+lssm_status lssm_logprobs(lssm_ctx* ctx, const void* logits, const uint32_t* targets, float* logp, float* entropy,
+                          float* lse, uint32_t* top_ids, float* top_logp, lssm_logprobs_dims dims);
+/* Gradient of logp and entropy with respect to the logits:
+ *   dlogits_j = g_logp ([j = t] - p_j) - g_entropy p_j (log p_j + entropy)
+ * lse and entropy (rows) are lssm_logprobs' outputs for the same logits; g_logp / g_entropy (rows)
+ * are the gradients of a scalar with respect to those outputs, null = none (not both); g_logp needs
+ * targets, g_entropy needs entropy. A LSSM_NO_TOKEN row takes nothing from g_logp, a row with lse -inf
+ * is 0, an id >= vocab makes the row NaN. lse, the alternatives and their order carry no gradient.
+ * dlogits is of grad_dtype, grad_stride elements apart (0 = vocab); it may be the logits themselves
+ * (same address, type and stride), and must not overlap them otherwise. */
+typedef struct {
+    uint32_t rows, vocab;
+    uint32_t dtype, grad_dtype;
+    uint64_t row_stride, grad_stride;
+} lssm_logprobs_grad_dims;
+lssm_status lssm_logprobs_backward(lssm_ctx* ctx, const void* logits, const uint32_t* targets, const float* lse,
+                                   const float* entropy, const float* g_logp, const float* g_entropy, void* dlogits,
+                                   lssm_logprobs_grad_dims dims);
+
+/* ---- quantised state cache (no reference counterpart: the reference keeps an fp32 state,
+ *      src/model/state.cpp:30-124) ----
+ * Holds the SSD states of `batch` sequences as 8- or 16-bit codes and the last tokens that the codes
+ * do not hold yet, so a decode step reads 1 or 2 bytes a state element and writes almost nothing;
+ * lssm_ssd_step_batched reads and writes 8. Six device arrays of the caller:
+ *   codes   (batch, H, P, N) int8 or int16    value = code * scale
+ *   scales  (batch, H, P) f32                 max |row of N| / 127 or / 32767
+ *   win_x   (batch, window, H * P) f16        x, B and dt of the tokens since the codes were written
+ *   win_B   (batch, window, G * N) f16
+ *   win_dt  (batch, H, window) f32
+ *   fill    (batch, H) u32                    tokens in the window, 0 .. window - 1
+ * A step whose token fills the window folds it into the codes (the state is rounded once in `window`
+ * tokens, to the nearest code, ties to even) and empties it. A row of N that holds a NaN or an
+ * infinity reads back as NaN; a row with max < 1.2e-38 * Q (Q = 127 or 32767) as 0.
+ * All arrays are batch-major, so a range of sequences is the arrays from its first sequence on.
+ * Steps that overlap on the GPU must not share a sequence. */
+#define LSSM_STATE_WINDOW_MAX 32u
+typedef struct {
+    uint32_t batch, H, P, N, n_groups;
+    uint32_t window;       /* 1 .. LSSM_STATE_WINDOW_MAX */
+    uint32_t bits;         /* 8 or 16 */
+    float dt_min, dt_max;
+    uint32_t has_D;
+} lssm_state_cache_dims;
+typedef struct {
+    void* codes;
+    float* scales;
+    void* win_x;
+    void* win_B;
+    float* win_dt;
+    uint32_t* fill;
+} lssm_state_cache;
+/* Bytes of the six arrays, in the order above (host only, no device needed). */
+lssm_status lssm_state_cache_bytes(lssm_state_cache_dims dims, uint64_t* out);
+/* Quantises fp32 states (batch, H, P, N) into the cache and empties its windows. */
+lssm_status lssm_state_cache_store(lssm_ctx* ctx, const float* state, lssm_state_cache cache,
+                                   lssm_state_cache_dims dims);
+/* The states as they stand (codes and window) into (batch, H, P, N) of state_dtype; the cache is not
+ * changed. A_log (H) f16 as in the steps. */
+lssm_status lssm_state_cache_load(lssm_ctx* ctx, lssm_state_cache cache, const void* A_log, void* state,
+                                  uint32_t state_dtype, lssm_state_cache_dims dims);
+/* lssm_ssd_step_batched over the cache: one decode token of dims.batch sequences, fp16 x (batch, H*P),
+ * B / C (batch, G*N), dt_raw (batch, H), dt_bias / A_log / D (H), fp16 y (batch, H*P). A_log must be
+ * the same at every step of a window. The call is the same whatever the windows hold, so a captured
+ * step may be replayed. */
+lssm_status lssm_ssd_step_cached(lssm_ctx* ctx, const void* x, const void* B, const void* C, const void* dt_raw,
+                                 const void* dt_bias, const void* A_log, const void* D_skip, lssm_state_cache cache,
+                                 void* y, lssm_state_cache_dims dims);
+
 /* ---- engine: .ssm model + session (the callers of the ops: the .cpp files of src/model and src/runtime) ---- */
 typedef struct lssm_model lssm_model;
 typedef struct lssm_session lssm_session;

@@ -562,4 +562,167 @@ lssm_status lssm_ssd_step_batched(lssm_ctx* ctx, const void* x, const void* B, c
     LAUNCH("ssd_step_batched", launch_ssd_step_ex(a, ctx->stream));
 }
 
+// ---- scoring ----------------------------------------------------------------
+// The checks of these ops need no device: they come before the context is looked at.
+static bool stride_bad(uint64_t stride, uint32_t n) { return stride && (stride < n || stride > (1ull << 40)); }
+static size_t dtype_bytes(uint32_t dt) { return dt == LSSM_DT_F32 ? 4 : 2; }
+
+lssm_status lssm_logprobs(lssm_ctx* ctx, const void* logits, const uint32_t* targets, float* logp, float* entropy,
+                          float* lse, uint32_t* top_ids, float* top_logp, lssm_logprobs_dims d) {
+    if (d.dtype > LSSM_DT_F32) return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: unsupported dtype code");
+    if (d.vocab == 0 || d.vocab > 0x7FFFFFFFu)
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: vocab must be 1 .. 2^31 - 1");
+    if (d.rows > 0x7FFFFFFFu) return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: rows must be below 2^31");
+    if (d.top_k > LSSM_TOP_K_MAX || d.top_k > d.vocab)
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: top_k must be at most %u and at most vocab", LSSM_TOP_K_MAX);
+    if (stride_bad(d.row_stride, d.vocab))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: row_stride must be 0 or vocab .. 2^40");
+    if ((top_ids != nullptr) != (d.top_k > 0) || (top_logp != nullptr) != (d.top_k > 0))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: top_ids and top_logp are given exactly when top_k > 0");
+    if (!logp && !entropy && !lse && !d.top_k) return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: no output given");
+    if (d.rows && !logits) return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: null logits");
+    if (d.rows && logp && !targets) return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: logp needs targets");
+    if (!aligned(logits, dtype_bytes(d.dtype)) || !aligned(targets, 4) || !aligned(logp, 4) || !aligned(entropy, 4) ||
+        !aligned(lse, 4) || !aligned(top_ids, 4) || !aligned(top_logp, 4))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: an array is not aligned to its element");
+    CHECK_CTX(ctx);
+    if (d.rows == 0) return finish_op(ctx, "logprobs");
+    LogprobsArgs a{};
+    a.logits = logits; a.targets = targets;
+    a.logp = logp; a.entropy = entropy; a.lse = lse; a.top_ids = top_ids; a.top_logp = top_logp;
+    a.rows = d.rows; a.vocab = d.vocab; a.top_k = d.top_k; a.dtype = d.dtype;
+    a.row_stride = d.row_stride ? d.row_stride : d.vocab;
+    LAUNCH("logprobs", launch_logprobs(a, ctx->stream));
+}
+
+lssm_status lssm_logprobs_backward(lssm_ctx* ctx, const void* logits, const uint32_t* targets, const float* lse,
+                                   const float* entropy, const float* g_logp, const float* g_entropy, void* dlogits,
+                                   lssm_logprobs_grad_dims d) {
+    if (d.dtype > LSSM_DT_F32 || d.grad_dtype > LSSM_DT_F32)
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: unsupported dtype code");
+    if (d.vocab == 0 || d.vocab > 0x7FFFFFFFu)
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: vocab must be 1 .. 2^31 - 1");
+    if (d.rows > 0x7FFFFFFFu) return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: rows must be below 2^31");
+    if (stride_bad(d.row_stride, d.vocab) || stride_bad(d.grad_stride, d.vocab))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: row_stride and grad_stride must be 0 or vocab .. 2^40");
+    if (!g_logp && !g_entropy) return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: no gradient given");
+    if (d.rows && (!logits || !lse || !dlogits))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: null logits, lse or dlogits");
+    if (d.rows && g_logp && !targets) return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: g_logp needs targets");
+    if (d.rows && g_entropy && !entropy) return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: g_entropy needs entropy");
+    if (!aligned(logits, dtype_bytes(d.dtype)) || !aligned(dlogits, dtype_bytes(d.grad_dtype)) || !aligned(targets, 4) ||
+        !aligned(lse, 4) || !aligned(entropy, 4) || !aligned(g_logp, 4) || !aligned(g_entropy, 4))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: an array is not aligned to its element");
+    LogprobsGradArgs a{};
+    a.logits = logits; a.targets = targets; a.lse = lse; a.entropy = entropy; a.g_logp = g_logp; a.g_entropy = g_entropy;
+    a.dlogits = dlogits;
+    a.rows = d.rows; a.vocab = d.vocab; a.dtype = d.dtype; a.grad_dtype = d.grad_dtype;
+    a.row_stride = d.row_stride ? d.row_stride : d.vocab;
+    a.grad_stride = d.grad_stride ? d.grad_stride : d.vocab;
+    const uint64_t es = dtype_bytes(d.dtype), gs = dtype_bytes(d.grad_dtype);
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(logits), g0 = reinterpret_cast<uintptr_t>(dlogits);
+    const uintptr_t x1 = x0 + ((uint64_t)(d.rows - 1) * a.row_stride + d.vocab) * es;
+    const uintptr_t g1 = g0 + ((uint64_t)(d.rows - 1) * a.grad_stride + d.vocab) * gs;
+    const bool same = x0 == g0 && d.dtype == d.grad_dtype && a.row_stride == a.grad_stride;
+    if (d.rows && !same && x0 < g1 && g0 < x1)
+        return fail(LSSM_ERR_INVALID_ARGUMENT,
+                    "logprobs_backward: dlogits overlaps the logits without being them (address, type and stride)");
+    CHECK_CTX(ctx);
+    if (d.rows == 0) return finish_op(ctx, "logprobs_backward");
+    LAUNCH("logprobs_backward", launch_logprobs_grad(a, ctx->stream));
+}
+
+// ---- quantised state cache ----------------------------------------------------
+static lssm_status state_cache_checks(const char* who, const lssm_state_cache_dims& d) {
+    if (d.bits != 8 && d.bits != 16) return fail(LSSM_ERR_INVALID_ARGUMENT, "%s: bits must be 8 or 16", who);
+    if (d.window < 1 || d.window > LSSM_STATE_WINDOW_MAX)
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "%s: window must be 1..%u", who, LSSM_STATE_WINDOW_MAX);
+    if (d.H % (d.n_groups ? d.n_groups : 1))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "%s: n_heads must be a multiple of n_groups", who);
+    if ((uint64_t)d.batch * d.H > 0x7FFFFFFFu || (uint64_t)d.H * d.P > 0x7FFFFFFFu ||
+        (uint64_t)d.n_groups * d.N > 0x7FFFFFFFu || d.P > 0xFFFFu || d.N > 0xFFFFu ||
+        (uint64_t)d.batch * d.H * d.P > 0x7FFFFFFFull * 8)
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "%s: batch, H, P or N too large", who);
+    return LSSM_OK;
+}
+
+static lssm_status state_cache_args(const char* who, const lssm_state_cache& c, const lssm_state_cache_dims& d,
+                                    StateCacheArgs* a) {
+    if (!c.codes || !c.scales || !c.win_x || !c.win_B || !c.win_dt || !c.fill)
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "%s: null cache array", who);
+    if (!aligned(c.codes, d.bits / 8) || !aligned(c.scales, 4) || !aligned(c.win_x, 2) || !aligned(c.win_B, 2) ||
+        !aligned(c.win_dt, 4) || !aligned(c.fill, 4))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "%s: a cache array is not aligned to its element", who);
+    *a = StateCacheArgs{};
+    a->codes = c.codes; a->scales = c.scales;
+    a->win_x = static_cast<__half*>(c.win_x); a->win_B = static_cast<__half*>(c.win_B);
+    a->win_dt = c.win_dt; a->fill = c.fill;
+    a->batch = d.batch; a->H = d.H; a->P = d.P; a->N = d.N; a->G = d.n_groups ? d.n_groups : 1;
+    a->W = d.window; a->bits = d.bits;
+    a->dt_min = d.dt_min; a->dt_max = d.dt_max; a->has_D = d.has_D;
+    return LSSM_OK;
+}
+
+lssm_status lssm_state_cache_bytes(lssm_state_cache_dims d, uint64_t* out) {
+    if (!out) return fail(LSSM_ERR_INVALID_ARGUMENT, "state_cache_bytes: null out");
+    if (lssm_status st = state_cache_checks("state_cache_bytes", d)) return st;
+    const uint64_t B = d.batch, H = d.H, P = d.P, N = d.N, W = d.window, G = d.n_groups ? d.n_groups : 1;
+    out[0] = B * H * P * N * (d.bits / 8);
+    out[1] = B * H * P * 4;
+    out[2] = B * W * H * P * 2;
+    out[3] = B * W * G * N * 2;
+    out[4] = B * H * W * 4;
+    out[5] = B * H * 4;
+    return LSSM_OK;
+}
+
+lssm_status lssm_state_cache_store(lssm_ctx* ctx, const float* state, lssm_state_cache cache,
+                                   lssm_state_cache_dims d) {
+    if (lssm_status st = state_cache_checks("state_cache_store", d)) return st;
+    StateCacheArgs a;
+    if (lssm_status st = state_cache_args("state_cache_store", cache, d, &a)) return st;
+    if (!state || !aligned(state, 4))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "state_cache_store: null or misaligned state");
+    a.state = const_cast<float*>(state);
+    CHECK_CTX(ctx);
+    if (!d.batch || !d.H || !d.P || !d.N) return finish_op(ctx, "state_cache_store");
+    LAUNCH("state_cache_store", launch_state_store(a, ctx->stream));
+}
+
+lssm_status lssm_state_cache_load(lssm_ctx* ctx, lssm_state_cache cache, const void* A_log, void* state,
+                                  uint32_t state_dtype, lssm_state_cache_dims d) {
+    if (lssm_status st = state_cache_checks("state_cache_load", d)) return st;
+    if (state_dtype > LSSM_DT_F32) return fail(LSSM_ERR_INVALID_ARGUMENT, "state_cache_load: unsupported dtype code");
+    StateCacheArgs a;
+    if (lssm_status st = state_cache_args("state_cache_load", cache, d, &a)) return st;
+    if (!state || !aligned(state, dtype_bytes(state_dtype)) || !A_log || !aligned(A_log, 2))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "state_cache_load: null or misaligned state or A_log");
+    a.A_log = static_cast<const __half*>(A_log);
+    a.state = state; a.state_dtype = state_dtype;
+    CHECK_CTX(ctx);
+    if (!d.batch || !d.H || !d.P || !d.N) return finish_op(ctx, "state_cache_load");
+    LAUNCH("state_cache_load", launch_state_load(a, ctx->stream));
+}
+
+lssm_status lssm_ssd_step_cached(lssm_ctx* ctx, const void* x, const void* B, const void* C, const void* dt_raw,
+                                 const void* dt_bias, const void* A_log, const void* D_skip, lssm_state_cache cache,
+                                 void* y, lssm_state_cache_dims d) {
+    if (lssm_status st = state_cache_checks("ssd_step_cached", d)) return st;
+    StateCacheArgs a;
+    if (lssm_status st = state_cache_args("ssd_step_cached", cache, d, &a)) return st;
+    if (!x || !B || !C || !dt_raw || !dt_bias || !A_log || !y || (d.has_D && !D_skip))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "ssd_step_cached: null array");
+    if (!aligned(x, 2) || !aligned(B, 2) || !aligned(C, 2) || !aligned(dt_raw, 2) || !aligned(dt_bias, 2) ||
+        !aligned(A_log, 2) || !aligned(D_skip, 2) || !aligned(y, 2))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "ssd_step_cached: an array is not aligned to its element");
+    a.x = static_cast<const __half*>(x); a.B = static_cast<const __half*>(B); a.C = static_cast<const __half*>(C);
+    a.dt_raw = static_cast<const __half*>(dt_raw); a.dt_bias = static_cast<const __half*>(dt_bias);
+    a.A_log = static_cast<const __half*>(A_log); a.D = static_cast<const __half*>(D_skip);
+    a.y = static_cast<__half*>(y);
+    a.x_bs = (uint64_t)d.H * d.P; a.bc_bs = (uint64_t)a.G * d.N; a.dt_bs = d.H; a.y_bs = a.x_bs;
+    CHECK_CTX(ctx);
+    if (!d.batch || !d.H || !d.P || !d.N) return finish_op(ctx, "ssd_step_cached");
+    LAUNCH("ssd_step_cached", launch_ssd_step_cached(a, ctx->stream));
+}
+
 }  // extern "C"

@@ -140,6 +140,41 @@ struct StepArgs {
 };
 cudaError_t launch_ssd_step_ex(const StepArgs& a, cudaStream_t s);
 
+// ---- scoring (k_logprobs.cu) --------------------------------------------------
+struct LogprobsArgs {
+    const void* logits; const uint32_t* targets;
+    float* logp; float* entropy; float* lse; uint32_t* top_ids; float* top_logp;
+    uint32_t rows, vocab, top_k, dtype;
+    uint64_t row_stride;
+};
+cudaError_t launch_logprobs(const LogprobsArgs& a, cudaStream_t s);
+struct LogprobsGradArgs {
+    const void* logits; const uint32_t* targets;
+    const float* lse; const float* entropy; const float* g_logp; const float* g_entropy;
+    void* dlogits;
+    uint32_t rows, vocab, dtype, grad_dtype;
+    uint64_t row_stride, grad_stride;
+};
+cudaError_t launch_logprobs_grad(const LogprobsGradArgs& a, cudaStream_t s);
+
+// ---- quantised state cache (k_state_cache.cu) ---------------------------------
+// `state`: the fp32 states that store reads, or the states of state_dtype that load writes.
+// Per-sequence strides in elements for x, B / C, dt_raw, y and the optional gate z (as StepArgs).
+struct StateCacheArgs {
+    void* codes; float* scales; __half* win_x; __half* win_B; float* win_dt; uint32_t* fill;
+    const __half* x; const __half* B; const __half* C; const __half* dt_raw;
+    const __half* dt_bias; const __half* A_log; const __half* D;
+    __half* y; const __half* z;
+    void* state; uint32_t state_dtype;
+    uint32_t batch, H, P, N, G, W, bits;
+    float dt_min, dt_max;
+    uint32_t has_D;
+    uint64_t x_bs, bc_bs, dt_bs, y_bs, z_bs;
+};
+cudaError_t launch_state_store(const StateCacheArgs& a, cudaStream_t s);
+cudaError_t launch_state_load(const StateCacheArgs& a, cudaStream_t s);
+cudaError_t launch_ssd_step_cached(const StateCacheArgs& a, cudaStream_t s);
+
 // ---- persistent decode kernel (k_decode_persist.cu) -------------------------
 struct PLayer {
     const uint8_t* in_w;       // in_proj packed (proj x dm/2); scales at in_w + proj*dm/2

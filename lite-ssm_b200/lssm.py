@@ -65,12 +65,33 @@ class SSDBatchedDims(C.Structure):
                 ("dt_dtype", u32), ("param_dtype", u32), ("y_dtype", u32)]
 
 
+class LogprobsDims(C.Structure):
+    _fields_ = [("rows", u32), ("vocab", u32), ("top_k", u32), ("dtype", u32), ("row_stride", u64)]
+
+
+class LogprobsGradDims(C.Structure):
+    _fields_ = [("rows", u32), ("vocab", u32), ("dtype", u32), ("grad_dtype", u32), ("row_stride", u64),
+                ("grad_stride", u64)]
+
+
+class StateCacheDims(C.Structure):
+    _fields_ = [("batch", u32), ("H", u32), ("P", u32), ("N", u32), ("n_groups", u32), ("window", u32),
+                ("bits", u32), ("dt_min", f32), ("dt_max", f32), ("has_D", u32)]
+
+
+class StateCachePtrs(C.Structure):
+    _fields_ = [(n, P) for n in ("codes", "scales", "win_x", "win_B", "win_dt", "fill")]
+
+
 class HParams(C.Structure):
     _fields_ = [(n, u32) for n in ("d_model", "n_layer", "d_state", "d_conv", "expand", "vocab_size", "n_heads",
                                    "d_head", "chunk_size", "default_dtype", "n_groups", "norm_before_gate")]
 
 
 DT_F16, DT_BF16, DT_F32 = 0, 1, 2
+NO_TOKEN = 0xFFFFFFFF    # a row without a target (lssm_logprobs)
+TOP_K_MAX = 32
+STATE_WINDOW_MAX = 32
 
 # (name, argtypes) for every exported function; restype is lssm_status (int) unless listed.
 _SIGS = {
@@ -109,6 +130,12 @@ _SIGS = {
     "lssm_ssd_chunked_f16": [P] + [P, sz] * 9 + [SSDDims],
     "lssm_ssd_step_f16": [P] + [P, sz] * 9 + [SSDStepDims],
     "lssm_ssd_chunked_batched": [P] * 10 + [SSDBatchedDims],
+    "lssm_logprobs": [P] * 8 + [LogprobsDims],
+    "lssm_logprobs_backward": [P] * 8 + [LogprobsGradDims],
+    "lssm_state_cache_bytes": [StateCacheDims, C.POINTER(u64)],
+    "lssm_state_cache_store": [P, P, StateCachePtrs, StateCacheDims],
+    "lssm_state_cache_load": [P, StateCachePtrs, P, P, u32, StateCacheDims],
+    "lssm_ssd_step_cached": [P] * 8 + [StateCachePtrs, P, StateCacheDims],
     "lssm_model_load": [P, C.c_char_p, C.POINTER(P)],
     "lssm_model_load_bytes": [P, P, sz, C.POINTER(P)],
     "lssm_model_synthesize": [P, C.POINTER(HParams), u64, C.c_int, C.POINTER(P)],
@@ -265,6 +292,11 @@ class Ctx:
     def batch_active(self) -> bool:
         return lib().lssm_batch_active(self.h) == 1
 
+    def set_stream(self, cuda_stream: int):
+        """Run on an external cudaStream_t (its handle as an int, e.g. torch's
+        `current_stream().cuda_stream`; 0 = the device's default stream)."""
+        check(lib().lssm_ctx_set_stream(self.h, cuda_stream))
+
     def stream(self) -> int:
         return lib().lssm_ctx_stream(self.h) or 0
 
@@ -309,6 +341,40 @@ class DeviceBuffer:
             self.free()
         except Exception:
             pass
+
+
+class DeviceView:
+    """Device memory that the caller owns (a torch tensor's data_ptr(), a part of a
+    DeviceBuffer), for calls that take a buffer. The caller keeps it alive."""
+
+    def __init__(self, ctx: Ctx, ptr: int):
+        self.ctx = ctx
+        self.ptr = P(ptr)
+
+
+class StateCache:
+    """The six device arrays of a quantised state cache (lssm_state_cache), empty windows and
+    zero states when made here."""
+
+    def __init__(self, ctx: Ctx, dims: StateCacheDims):
+        n = (u64 * 6)()
+        check(lib().lssm_state_cache_bytes(dims, n))
+        self.buffers = [DeviceBuffer(ctx, int(k)) for k in n]
+        for b in self.buffers:
+            b.zero()
+        self.ptrs = StateCachePtrs(*(b.ptr for b in self.buffers))
+
+    @classmethod
+    def wrap(cls, codes: int, scales: int, win_x: int, win_B: int, win_dt: int, fill: int):
+        """A cache over device arrays that the caller owns, by their addresses."""
+        c = cls.__new__(cls)
+        c.buffers = []
+        c.ptrs = StateCachePtrs(codes, scales, win_x, win_B, win_dt, fill)
+        return c
+
+
+def _ptr(x):
+    return None if x is None else x.ptr
 
 
 class Ops:
@@ -404,6 +470,29 @@ class Ops:
     def ssd_chunked_batched(self, X, B, Cm, dt_raw, dt_bias, A_log, D_skip, Y, state_io, dims: SSDBatchedDims):
         self._call("lssm_ssd_chunked_batched", X.ptr, B.ptr, Cm.ptr, dt_raw.ptr, dt_bias.ptr, A_log.ptr, D_skip.ptr,
                    Y.ptr, state_io.ptr, dims)
+
+    def logprobs(self, logits, targets, logp, entropy, lse, top_ids, top_logp, dims: LogprobsDims):
+        """Log probabilities of given tokens, entropy, log-sum-exp and the top alternatives of rows of
+        logits (lssm_logprobs). Buffers; None for an output that is not wanted."""
+        self._call("lssm_logprobs", *map(_ptr, (logits, targets, logp, entropy, lse, top_ids, top_logp)), dims)
+
+    def logprobs_backward(self, logits, targets, lse, entropy, g_logp, g_entropy, dlogits, dims: LogprobsGradDims):
+        """Gradient of logprobs' logp and entropy with respect to the logits (lssm_logprobs_backward)."""
+        self._call("lssm_logprobs_backward", *map(_ptr, (logits, targets, lse, entropy, g_logp, g_entropy, dlogits)),
+                   dims)
+
+    def state_cache_store(self, state, cache: StateCache, dims: StateCacheDims):
+        """Quantise fp32 states into the cache and empty its windows (lssm_state_cache_store)."""
+        self._call("lssm_state_cache_store", _ptr(state), cache.ptrs, dims)
+
+    def state_cache_load(self, cache: StateCache, A_log, state, state_dtype: int, dims: StateCacheDims):
+        """The cached states as they stand, in state_dtype (lssm_state_cache_load)."""
+        self._call("lssm_state_cache_load", cache.ptrs, _ptr(A_log), _ptr(state), state_dtype, dims)
+
+    def ssd_step_cached(self, x, B, Cm, dt_raw, dt_bias, A_log, D_skip, cache: StateCache, y, dims: StateCacheDims):
+        """One decode token of a batch of sequences over the cache (lssm_ssd_step_cached)."""
+        self._call("lssm_ssd_step_cached", *map(_ptr, (x, B, Cm, dt_raw, dt_bias, A_log, D_skip)), cache.ptrs, _ptr(y),
+                   dims)
 
 
 class Model:
