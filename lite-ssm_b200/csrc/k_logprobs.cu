@@ -280,7 +280,8 @@ __device__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t c1, uint32_t tk
             const uint32_t c = c0 + sh.sel[q / per] + (q % per) * LP_THREADS;
             if (c >= c1) continue;
             const uint4 raw = row.chunk(c);
-            if (chunk_max(raw, T()) < bv) continue;
+            const float cm = chunk_max(raw, T());
+            if (ties ? cm < bv : !(cm > bv)) continue;
             float x[VEC];
             chunk_values<T>(raw, x);
             const int64_t e = row.index(c);
@@ -293,10 +294,11 @@ __device__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t c1, uint32_t tk
             }
         }
     };
-    collect(true);
+    const bool level = sh.nsel > LP_THREADS / 4;   // many threads reach the bound: a masked or constant row
+    if (!level) collect(true);
     __syncthreads();
     uint32_t n = sh.count;
-    if (n > LP_CAND) {
+    if (level || n > LP_CAND) {
         // Many equal to the bound (masked or constant rows): those above it first, then of the
         // equal ones as many as are missing, in the order of their index.
         __syncthreads();
@@ -396,11 +398,7 @@ __global__ void __launch_bounds__(LP_THREADS) k_logprobs(LogprobsArgs a, uint32_
     }
     Sums<T> sum;
     float tmax = -INFINITY;
-    for (uint32_t c = c0 + tid; c < c1; c += LP_THREADS * LP_GROUP) {
-        uint4 w[LP_GROUP];
-#pragma unroll
-        for (int g = 0; g < LP_GROUP; ++g)
-            w[g] = c + g * LP_THREADS < c1 ? row.chunk(c + g * LP_THREADS) : Row<T>::nothing();
+    auto group = [&](const uint4 (&w)[LP_GROUP]) {
         float gm = chunk_max(w[0], T());
 #pragma unroll
         for (int g = 1; g < LP_GROUP; ++g) gm = fmaxf(gm, chunk_max(w[g], T()));
@@ -408,6 +406,29 @@ __global__ void __launch_bounds__(LP_THREADS) k_logprobs(LogprobsArgs a, uint32_
         sum.follow(gm);
 #pragma unroll
         for (int g = 0; g < LP_GROUP; ++g) sum.chunk(w[g]);
+    };
+    // whole groups of whole chunks first: chunks [inner, outer) lie inside the row
+    const uint32_t inner = max(c0, row.lead ? 1u : 0u), outer = min(c1, (row.V + row.lead) / Row<T>::VEC);
+    constexpr uint32_t STRIDE = LP_THREADS * LP_GROUP;
+    uint32_t c = c0 + tid;
+    if (c < inner) {
+        const uint4 w[LP_GROUP] = {row.chunk(c), Row<T>::nothing(), Row<T>::nothing(), Row<T>::nothing()};
+        group(w);
+        c += LP_THREADS;
+    }
+    const uint4* at = reinterpret_cast<const uint4*>(row.x - row.lead) + c;
+    for (; c + 3 * LP_THREADS < outer; c += STRIDE, at += STRIDE) {
+        uint4 w[LP_GROUP];
+#pragma unroll
+        for (int g = 0; g < LP_GROUP; ++g) w[g] = __ldg(at + g * LP_THREADS);
+        group(w);
+    }
+    if (c < c1) {
+        uint4 w[LP_GROUP];
+#pragma unroll
+        for (int g = 0; g < LP_GROUP; ++g)
+            w[g] = c + g * LP_THREADS < c1 ? row.chunk(c + g * LP_THREADS) : Row<T>::nothing();
+        group(w);
     }
     // the CTA's sums against its maximum
     float m = warp_max(tmax);
