@@ -21,8 +21,9 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
-constexpr int LP_GROUP = 4;          // 16-byte loads a thread has in flight
+constexpr int LP_GROUP = 4;          // 16-byte loads that a thread has on their way while it works on as many
 constexpr int LP_CAND = 1024;        // candidates for the top entries that a CTA holds
+constexpr int LP_HITS = 256;         // chunks that may hold one
 constexpr int LP_CLUSTER_MAX = 8;
 constexpr uint32_t FULL = 0xffffffffu;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
@@ -52,12 +53,16 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
-// Two fp32 lanes in one instruction.
+// Two fp32 lanes in one instruction, as the two halves of a 64-bit register.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
-    return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
 }
 __device__ __forceinline__ float2 unpack2(uint64_t v) {
-    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
 }
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t d;
@@ -85,17 +90,21 @@ struct Row {
         V = vocab;
         chunks = (uint32_t)(((uint64_t)vocab + lead + VEC - 1) / VEC);
     }
+    // Chunks [inner, outer) lie inside the row.
+    __device__ __forceinline__ uint32_t inner() const { return lead ? 1u : 0u; }
+    __device__ __forceinline__ uint32_t outer() const { return (V + lead) / VEC; }
+    __device__ __forceinline__ const uint4* base() const { return reinterpret_cast<const uint4*>(x - lead); }
     __device__ __forceinline__ int64_t index(uint32_t c) const { return (int64_t)c * VEC - lead; }
     static __device__ __forceinline__ T lowest() {
         if constexpr (sizeof(T) == 4) return -INFINITY;
         else { const uint16_t b = std::is_same<T, __half>::value ? 0xFC00 : 0xFF80; T v; memcpy(&v, &b, 2); return v; }
     }
     __device__ __forceinline__ uint4 chunk(uint32_t c) const {
-        const int64_t e = index(c);
         uint4 r;
-        if (e >= 0 && e + VEC <= (int64_t)V) {
-            r = __ldg(reinterpret_cast<const uint4*>(x + e));
+        if (c >= inner() && c < outer()) {
+            r = __ldg(base() + c);
         } else {
+            const int64_t e = index(c);
             T t[VEC];
 #pragma unroll
             for (int i = 0; i < VEC; ++i) t[i] = e + i >= 0 && e + i < (int64_t)V ? x[e + i] : lowest();
@@ -148,6 +157,10 @@ __device__ __forceinline__ void chunk_values(uint4 c, float (&v)[16 / sizeof(T)]
     }
 }
 
+__device__ __forceinline__ float load_one(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ float load_one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float load_one(const float* p) { return *p; }
+
 // Running sums of one thread: with z = (x - ref) log2 e, s = sum 2^z and u = sum 2^z z, two lanes
 // each. For fp16, whose range allows it, z is one fma against refL = ref log2 e as rounded; `slip`
 // gives back what that rounding moved.
@@ -179,10 +192,11 @@ struct Sums {
         s2 = pack2(s.x, s.y);
         u2 = pack2(u.x, u.y);
     }
-    __device__ __forceinline__ void add(float z0, float z1) {
-        const uint64_t e = pack2(ex2(z0), ex2(z1));
+    __device__ __forceinline__ void add(uint64_t z) {
+        const float2 f = unpack2(z);
+        const uint64_t e = pack2(ex2(f.x), ex2(f.y));
         s2 = add2(s2, e);
-        u2 = fma2(e, pack2(z0, z1), u2);
+        u2 = fma2(e, z, u2);
     }
     __device__ __forceinline__ void chunk(uint4 c) {
         const uint32_t w[4] = {c.x, c.y, c.z, c.w};
@@ -196,8 +210,7 @@ struct Sums {
                     __half2 h;
                     memcpy(&h, &w[i], 4);
                     const float2 f = __half22float2(__hmax2_nan(h, low));
-                    const float2 z = unpack2(fma2(pack2(f.x, f.y), l2, r2));
-                    add(z.x, z.y);
+                    add(fma2(pack2(f.x, f.y), l2, r2));
                 }
             } else {
                 // nothing but -inf and values near the lowest so far: they have to be told apart
@@ -205,7 +218,7 @@ struct Sums {
                 for (int i = 0; i < 4; ++i) {
                     const float2 f = to_float2(w[i], T());
                     const float2 z = unpack2(fma2(pack2(f.x, f.y), l2, r2));
-                    add(max_or_nan(z.x, -300.0f), max_or_nan(z.y, -300.0f));
+                    add(pack2(max_or_nan(z.x, -300.0f), max_or_nan(z.y, -300.0f)));
                 }
             }
         } else {
@@ -213,13 +226,13 @@ struct Sums {
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
                 for (int i = 0; i < 4; i += 2)
-                    add(max_or_nan((__uint_as_float(w[i]) - r) * LOG2E, -300.0f),
-                        max_or_nan((__uint_as_float(w[i + 1]) - r) * LOG2E, -300.0f));
+                    add(pack2(max_or_nan((__uint_as_float(w[i]) - r) * LOG2E, -300.0f),
+                              max_or_nan((__uint_as_float(w[i + 1]) - r) * LOG2E, -300.0f)));
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 f = to_float2(w[i], T());
-                    add(max_or_nan((f.x - r) * LOG2E, -300.0f), max_or_nan((f.y - r) * LOG2E, -300.0f));
+                    add(pack2(max_or_nan((f.x - r) * LOG2E, -300.0f), max_or_nan((f.y - r) * LOG2E, -300.0f)));
                 }
             }
         }
@@ -228,44 +241,45 @@ struct Sums {
 
 struct LpShared {
     uint64_t cand[LP_CAND + LSSM_TOP_K_MAX];
-    uint64_t list[LSSM_TOP_K_MAX];                    // the CTA's top entries, in order (0: none)
-    uint64_t all[LP_CLUSTER_MAX * LSSM_TOP_K_MAX];    // the cluster's (first CTA)
-    float m, s, u;                                    // the CTA's sums against its maximum
-    float red[3][LP_WARPS];
-    uint32_t maxima[LP_WARPS * 4];
-    uint32_t count, nsel, wsum[LP_WARPS];
+    uint4 hit[LP_HITS];                               // chunks that hold an entry at or above the bound
+    uint32_t hit_at[LP_HITS];
+    // what the CTAs of a cluster send to the first one: sums against their maxima, and their top entries in
+    // order, 0 behind the last
+    float m[LP_CLUSTER_MAX], s[LP_CLUSTER_MAX], u[LP_CLUSTER_MAX];
+    uint64_t list[LP_CLUSTER_MAX][LSSM_TOP_K_MAX];
+    float red[2][LP_WARPS];
+    alignas(16) uint32_t maxima[LP_WARPS * 4];        // the four largest thread maxima of every warp (order_key)
+    uint32_t count, nhits, nsel, bound, wsum[LP_WARPS];
+    uint64_t wbest[LP_WARPS];
     uint8_t sel[LP_THREADS];
 };
 
-// The CTA's largest K entries of chunks [c0, c1) into sh.list. `tkey`: this thread's largest (order_key).
-//
-// A value that at least K entries reach: the K-th largest of the four largest thread maxima of
-// every warp. Only threads whose maximum reaches it can hold one of the top K, so only their chunks
-// (about K / 256 of the slice, still in L2) are read again. The entries that reach the bound are
-// counted, stored and ranked against one another by value and index.
-template <typename T>
-__device__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t c1, uint32_t tkey, uint32_t K, LpShared& sh) {
-    constexpr int VEC = 16 / sizeof(T);
-    const uint32_t tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-    uint32_t mine = tkey;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const uint32_t top = __reduce_max_sync(FULL, mine);
-        if (lane == 0) sh.maxima[wid * 4 + r] = top;
-        if ((int)lane == __ffs(__ballot_sync(FULL, mine == top)) - 1) mine = 0;
-    }
-    if (tid == 0) { sh.count = 0; sh.nsel = 0; }
-    if (tid < LSSM_TOP_K_MAX) sh.list[tid] = 0;
-    __syncthreads();
-    // the K-th largest of the 32: the one with K - 1 before it
-    const uint32_t v = sh.maxima[lane];
+// The first warp: of K of the 32 warp maxima the least, the largest K up to an order among values within 32
+// steps of one another (for which every entry is made different by its place in the last bits).
+__device__ __forceinline__ void find_bound(uint32_t K, LpShared& sh) {
+    const uint32_t lane = threadIdx.x & 31, v = sh.maxima[lane], vr = (v & ~31u) | lane;
     uint32_t before = 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const uint32_t o = sh.maxima[i];
-        before += o > v || (o == v && i < (int)lane);
+    for (uint32_t i = 0; i < 32; i += 4) {
+        const uint4 o = *reinterpret_cast<const uint4*>(&sh.maxima[i]);
+        before += (((o.x & ~31u) | i) > vr) + (((o.y & ~31u) | (i + 1)) > vr) + (((o.z & ~31u) | (i + 2)) > vr) +
+                  (((o.w & ~31u) | (i + 3)) > vr);
     }
-    const uint32_t bound = __shfl_sync(FULL, v, __ffs(__ballot_sync(FULL, before == K - 1)) - 1);
+    const uint32_t least = __reduce_min_sync(FULL, before < K ? v : ~0u);
+    if (lane == 0) sh.bound = least;
+}
+
+// The CTA's largest K entries of chunks [c0, c1), in order, into `list`. `tkey`: this thread's largest entry.
+//
+// sh.bound is a value that at least K entries reach. Only threads whose maximum reaches it can hold one of the
+// top K, so only their chunks (about K / 256 of the slice, still in L2) are read again, and of those that reach
+// it the elements. What reaches the bound is ranked by value and index.
+template <typename T>
+__device__ __forceinline__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t c1, uint32_t tkey, uint32_t K, LpShared& sh,
+                                        uint64_t* list) {
+    constexpr int VEC = 16 / sizeof(T);
+    const uint32_t tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+    const uint32_t bound = sh.bound;
     const bool chosen = tkey >= bound;
     const uint32_t votes = __ballot_sync(FULL, chosen);
     uint32_t at = 0;
@@ -273,41 +287,51 @@ __device__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t c1, uint32_t tk
     at = __shfl_sync(FULL, at, 0) + __popc(votes & ((1u << lane) - 1));
     if (chosen) sh.sel[at] = (uint8_t)tid;
     __syncthreads();
-    const uint32_t per = (c1 - c0 + LP_THREADS - 1) / LP_THREADS, items = sh.nsel * per;
+    const uint32_t nsel = sh.nsel;
     const float bv = key_value(bound);
+    const bool level = nsel > LP_THREADS / 4;   // many threads reach the bound: a masked or constant row
     auto collect = [&](bool ties) {
-        for (uint32_t q = tid; q < items; q += LP_THREADS) {
-            const uint32_t c = c0 + sh.sel[q / per] + (q % per) * LP_THREADS;
-            if (c >= c1) continue;
-            const uint4 raw = row.chunk(c);
-            const float cm = chunk_max(raw, T());
-            if (ties ? cm < bv : !(cm > bv)) continue;
-            float x[VEC];
-            chunk_values<T>(raw, x);
-            const int64_t e = row.index(c);
+        // a warp takes four chosen threads at a time, a lane one of their chunks
+        for (uint32_t i = wid * 4; i < nsel; i += LP_WARPS * 4)
+            for (uint32_t k = lane * LP_THREADS; c0 + k < c1; k += 32 * LP_THREADS) {
+                uint4 w[4];
+                uint32_t c[4];
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const uint32_t k = order_key(x[i]);
-                if (k < bound || (k == bound && !ties) || e + i < 0 || e + i >= (int64_t)row.V) continue;
-                const uint32_t p = atomicAdd(&sh.count, 1u);
-                if (p < LP_CAND) sh.cand[p] = rank_key(k, (uint32_t)(e + i));
+                for (int g = 0; g < 4; ++g) {
+                    c[g] = i + g < nsel ? c0 + k + sh.sel[i + g] : c1;
+                    if (c[g] < c1) w[g] = row.chunk(c[g]);
+                }
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    if (c[g] >= c1) continue;
+                    const float cm = chunk_max(w[g], T());
+                    if (ties ? cm < bv : cm <= bv) continue;
+                    const uint32_t p = atomicAdd(&sh.nhits, 1u);
+                    if (p < LP_HITS) { sh.hit[p] = w[g]; sh.hit_at[p] = c[g]; }
+                }
             }
-        }
-    };
-    const bool level = sh.nsel > LP_THREADS / 4;   // many threads reach the bound: a masked or constant row
-    if (!level) collect(true);
-    __syncthreads();
-    uint32_t n = sh.count;
-    if (level || n > LP_CAND) {
-        // Many equal to the bound (masked or constant rows): those above it first, then of the
-        // equal ones as many as are missing, in the order of their index.
         __syncthreads();
-        if (tid == 0) sh.count = 0;
+        const uint32_t nh = min(sh.nhits, (uint32_t)LP_HITS);
+        for (uint32_t q = tid; q < nh * VEC; q += LP_THREADS) {
+            const int64_t e = row.index(sh.hit_at[q / VEC]) + q % VEC;
+            const uint32_t k = order_key(load_one(reinterpret_cast<const T*>(sh.hit) + q));
+            if (k < bound || (k == bound && !ties) || e < 0 || e >= (int64_t)row.V) continue;
+            const uint32_t p = atomicAdd(&sh.count, 1u);
+            if (p < LP_CAND) sh.cand[p] = rank_key(k, (uint32_t)e);
+        }
+        __syncthreads();
+    };
+    if (!level) collect(true);
+    uint32_t n = sh.count;
+    if (level || sh.nhits > LP_HITS || n > LP_CAND) {
+        // Many equal to the bound: those above it first, then of the equal ones as many as are missing,
+        // in the order of their index.
+        __syncthreads();
+        if (tid == 0) { sh.count = 0; sh.nhits = 0; }
         __syncthreads();
         collect(false);
-        __syncthreads();
         n = sh.count;
-        if (n <= LP_CAND) {
+        if (sh.nhits <= LP_HITS && n <= LP_CAND) {
             uint32_t have = n;
             for (uint32_t c = c0; c < c1 && have < K; c += LP_THREADS) {
                 const uint32_t mc = c + tid;
@@ -363,144 +387,161 @@ __device__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t c1, uint32_t tk
                     best = w > best ? w : best;
                 }
                 __syncthreads();
-                if (lane == 0) sh.all[wid] = best;
+                if (lane == 0) sh.wbest[wid] = best;
                 __syncthreads();
-                last = sh.all[0];
-                for (int w = 1; w < LP_WARPS; ++w) last = sh.all[w] > last ? sh.all[w] : last;
+                last = sh.wbest[0];
+                for (int w = 1; w < LP_WARPS; ++w) last = sh.wbest[w] > last ? sh.wbest[w] : last;
                 if (tid == 0) sh.cand[k] = last;
             }
             n = K;
         }
         __syncthreads();
     }
-    for (uint32_t i = tid; i < n; i += LP_THREADS) {
-        const uint64_t k = sh.cand[i];
+    // eight threads a candidate count those before it
+    for (uint32_t i = tid / 8; i < (n + 3) / 4 * 4; i += LP_THREADS / 8) {
+        const uint64_t k = i < n ? sh.cand[i] : ~0ull;
         uint32_t r = 0;
-        for (uint32_t j = 0; j < n; ++j) r += sh.cand[j] > k;
-        if (r < K) sh.list[r] = k;
+#pragma unroll 4
+        for (uint32_t j = tid % 8; j < n; j += 8) r += sh.cand[j] > k;
+        r += __shfl_xor_sync(FULL, r, 1);
+        r += __shfl_xor_sync(FULL, r, 2);
+        r += __shfl_xor_sync(FULL, r, 4);
+        if (tid % 8 == 0 && i < n && r < K) list[r] = k;
     }
+    if (tid >= n && tid < LSSM_TOP_K_MAX) list[tid] = 0;
 }
 
 // One CTA, or a cluster of them over slices of the vocabulary, per row; one pass over the logits.
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) k_logprobs(LogprobsArgs a, uint32_t nc) {
+__global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(LogprobsArgs a, uint32_t nc) {
     __shared__ LpShared sh;
     const uint32_t tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const uint32_t r = blockIdx.x / nc, part = blockIdx.x % nc;
     const Row<T> row(a.logits, (uint64_t)r * a.row_stride, a.vocab);
     const uint32_t per = (row.chunks + nc - 1) / nc;
     const uint32_t c0 = min(row.chunks, part * per), c1 = min(row.chunks, c0 + per);
+    if (nc > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA runs
     uint32_t target = LSSM_NO_TOKEN;
-    float xt = 0.0f;
-    if (part == 0 && tid == 0 && a.logp) {
-        target = a.targets[r];
-        if (target < a.vocab) xt = load_any(row.x, target, a.dtype);
-    }
+    if (part == 0 && tid == LP_THREADS - 32 && a.logp) target = a.targets[r];
     Sums<T> sum;
     float tmax = -INFINITY;
-    auto group = [&](const uint4 (&w)[LP_GROUP]) {
-        float gm = chunk_max(w[0], T());
+    // This thread's chunks c0 + tid, + LP_THREADS, ...: groups of LP_GROUP that lie inside the row, the next one
+    // loaded before this one is worked on, and one by one what is left of the slice's ends.
+    const uint32_t inner = row.inner(), outer = min(c1, row.outer());
+    constexpr uint32_t STRIDE = LP_THREADS * LP_GROUP;
+    uint32_t c = c0 + tid;
+    auto single = [&](uint32_t k) {
+        const uint4 w = row.chunk(k);
+        const float gm = chunk_max(w, T());
+        tmax = fmaxf(tmax, gm);
+        sum.follow(gm);
+        sum.chunk(w);
+    };
+    const bool head = c < inner;
+    if (head) c += LP_THREADS;
+    uint32_t groups = c < outer ? (outer - c + LP_THREADS - 1) / LP_THREADS / LP_GROUP : 0;
+    const uint4* at = row.base() + c;
+    auto load = [&](uint4 (&d)[LP_GROUP]) {
 #pragma unroll
-        for (int g = 1; g < LP_GROUP; ++g) gm = fmaxf(gm, chunk_max(w[g], T()));
+        for (int g = 0; g < LP_GROUP; ++g) d[g] = __ldg(at + g * LP_THREADS);
+        at += STRIDE;
+    };
+    auto work = [&](const uint4 (&d)[LP_GROUP]) {
+        float gm = chunk_max(d[0], T());
+#pragma unroll
+        for (int g = 1; g < LP_GROUP; ++g) gm = fmaxf(gm, chunk_max(d[g], T()));
         tmax = fmaxf(tmax, gm);
         sum.follow(gm);
 #pragma unroll
-        for (int g = 0; g < LP_GROUP; ++g) sum.chunk(w[g]);
+        for (int g = 0; g < LP_GROUP; ++g) sum.chunk(d[g]);
     };
-    // whole groups of whole chunks first: chunks [inner, outer) lie inside the row
-    const uint32_t inner = max(c0, row.lead ? 1u : 0u), outer = min(c1, (row.V + row.lead) / Row<T>::VEC);
-    constexpr uint32_t STRIDE = LP_THREADS * LP_GROUP;
-    uint32_t c = c0 + tid;
-    if (c < inner) {
-        const uint4 w[LP_GROUP] = {row.chunk(c), Row<T>::nothing(), Row<T>::nothing(), Row<T>::nothing()};
-        group(w);
-        c += LP_THREADS;
+    uint4 w[LP_GROUP], next[LP_GROUP];
+    if (groups) load(w);
+    if (head) single(c - LP_THREADS);
+    for (uint32_t k = c + groups * STRIDE; k < c1; k += LP_THREADS) single(k);
+    while (groups) {
+        if (--groups) load(next);
+        work(w);
+        if (!groups) break;
+        if (--groups) load(w);
+        work(next);
     }
-    const uint4* at = reinterpret_cast<const uint4*>(row.x - row.lead) + c;
-    for (; c + 3 * LP_THREADS < outer; c += STRIDE, at += STRIDE) {
-        uint4 w[LP_GROUP];
+    // the largest thread maxima of every warp, the CTA's maximum, and the sums against it
+    const uint32_t tkey = order_key(tmax), K = a.top_k;
+    uint32_t mine = tkey;
 #pragma unroll
-        for (int g = 0; g < LP_GROUP; ++g) w[g] = __ldg(at + g * LP_THREADS);
-        group(w);
+    for (int q = 0; q < 4; ++q) {
+        const uint32_t top = __reduce_max_sync(FULL, mine);
+        if (lane == 0) sh.maxima[wid * 4 + q] = top;
+        if ((int)lane == __ffs(__ballot_sync(FULL, mine == top)) - 1) mine = 0;
     }
-    if (c < c1) {
-        uint4 w[LP_GROUP];
-#pragma unroll
-        for (int g = 0; g < LP_GROUP; ++g)
-            w[g] = c + g * LP_THREADS < c1 ? row.chunk(c + g * LP_THREADS) : Row<T>::nothing();
-        group(w);
-    }
-    // the CTA's sums against its maximum
-    float m = warp_max(tmax);
-    if (lane == 0) sh.red[0][wid] = m;
+    if (tid == 0) { sh.count = 0; sh.nhits = 0; sh.nsel = 0; }
     __syncthreads();
-    m = sh.red[0][0];
-#pragma unroll
-    for (int w = 1; w < LP_WARPS; ++w) m = fmaxf(m, sh.red[0][w]);
+    float m = key_value(__reduce_max_sync(FULL, sh.maxima[lane]));
+    if (K && wid == 0) find_bound(K, sh);
     float2 s2 = unpack2(sum.s2), u2 = unpack2(sum.u2);
     float s = s2.x + s2.y, u = u2.x + u2.y;
     if (sum.ref > -INFINITY && m < INFINITY) Sums<T>::shift((sum.ref - m) * LOG2E + sum.slip(), s, u);
     s = warp_sum(s);
     u = warp_sum(u);
-    __syncthreads();
-    if (lane == 0) { sh.red[1][wid] = s; sh.red[2][wid] = u; }
-    if (a.top_k) cta_top(row, c0, c1, order_key(tmax), a.top_k, sh);
+    if (lane == 0) { sh.red[0][wid] = s; sh.red[1][wid] = u; }
     __syncthreads();
     s = u = 0.0f;
 #pragma unroll
-    for (int w = 0; w < LP_WARPS; ++w) { s += sh.red[1][w]; u += sh.red[2][w]; }
-    const uint32_t K = a.top_k;
-    const uint64_t* lists = sh.list;
+    for (int w = 0; w < LP_WARPS; ++w) { s += sh.red[0][w]; u += sh.red[1][w]; }
+    if (K) cta_top(row, c0, c1, tkey, K, sh, sh.list[part]);
+    __syncthreads();
     if (nc > 1) {
-        // the slices' sums and lists meet in the first CTA of the cluster
-        cg::cluster_group cl = cg::this_cluster();
-        if (tid == 0) { sh.m = m; sh.s = s; sh.u = u; }
-        cl.sync();
-        if (part == 0) {
-            float mm = m;
-            for (uint32_t p = 1; p < nc; ++p) mm = fmaxf(mm, *cl.map_shared_rank(&sh.m, p));
-            float ss = 0.0f, uu = 0.0f;
-            for (uint32_t p = 0; p < nc; ++p) {
-                const float pm = *cl.map_shared_rank(&sh.m, p);
-                float ps = *cl.map_shared_rank(&sh.s, p), pu = *cl.map_shared_rank(&sh.u, p);
-                if (pm > -INFINITY && mm < INFINITY) Sums<T>::shift((pm - mm) * LOG2E, ps, pu);
-                ss += ps;
-                uu += pu;
+        // the slices' sums and lists meet in the first CTA of the cluster, whose CTAs all run by now
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        if (part != 0 && tid < 32) {
+            cg::cluster_group cl = cg::this_cluster();
+            if (tid < K) *cl.map_shared_rank(&sh.list[part][tid], 0) = sh.list[part][tid];
+            if (tid == 0) {
+                *cl.map_shared_rank(&sh.m[part], 0) = m;
+                *cl.map_shared_rank(&sh.s[part], 0) = s;
+                *cl.map_shared_rank(&sh.u[part], 0) = u;
             }
-            m = mm; s = ss; u = uu;
-            for (uint32_t i = tid; i < nc * K; i += LP_THREADS) sh.all[i] = *cl.map_shared_rank(&sh.list[i % K], i / K);
         }
-        cl.sync();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         if (part != 0) return;
-        lists = sh.all;
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        const float pm = lane == 0 ? m : lane < nc ? sh.m[lane] : -INFINITY;
+        float ps = lane == 0 ? s : lane < nc ? sh.s[lane] : 0.0f, pu = lane == 0 ? u : lane < nc ? sh.u[lane] : 0.0f;
+        m = warp_max(pm);
+        if (pm > -INFINITY && m < INFINITY) Sums<T>::shift((pm - m) * LOG2E, ps, pu);
+        s = warp_sum(ps);
+        u = warp_sum(pu);
     }
     const bool none = m == -INFINITY && !(s != s);
     const float ls = m == INFINITY ? __int_as_float(0x7FC00000) : logf(s);
-    if (tid == 0) {
+    if (tid == LP_THREADS - 32) {   // a warp that has no alternative to write where there is one list
         if (a.lse) a.lse[r] = none ? -INFINITY : m + ls;
         if (a.entropy) a.entropy[r] = none ? 0.0f : ls - LN2 * (u / s);
         if (a.logp) {
             float v = 0.0f;
             if (target != LSSM_NO_TOKEN)
-                v = target >= a.vocab ? __int_as_float(0x7FC00000) : none ? -INFINITY : (xt - m) - ls;
+                v = target >= a.vocab ? __int_as_float(0x7FC00000) : none ? -INFINITY : (load_one(row.x + target) - m) - ls;
             a.logp[r] = v;
         }
     }
-    for (uint32_t i = tid; i < nc * K; i += LP_THREADS) {
-        const uint64_t k = lists[i];
-        if (!k) continue;
-        // its place: the entries before it in its own list and in every other (each in order)
-        uint32_t place = i % K;
-        for (uint32_t p = 0; p < nc && place < K; ++p) {
-            if (p == i / K) continue;
-            uint32_t lo = 0, hi = K;
-            while (lo < hi) {
-                const uint32_t mid = (lo + hi) / 2;
-                if (lists[p * K + mid] > k) lo = mid + 1; else hi = mid;
+    if (wid < nc && lane < K) {
+        // entry `lane` of list `wid`; its place: the entries before it, in its own list and in the others
+        const uint64_t k = sh.list[wid][lane];
+        uint32_t place = lane;
+        if (nc > 1) {
+#pragma unroll
+            for (uint32_t p = 0; p < LP_CLUSTER_MAX; ++p) {
+                if (p >= nc || p == wid) continue;
+                uint32_t lo = 0;
+#pragma unroll
+                for (uint32_t step = 16; step; step >>= 1)
+                    if (lo + step <= K && sh.list[p][lo + step - 1] > k) lo += step;
+                if (lo < K && sh.list[p][lo] > k) ++lo;
+                place += lo;
             }
-            place += lo;
         }
-        if (place < K) {
+        if (k && place < K) {
             a.top_ids[(uint64_t)r * K + place] = ~(uint32_t)k;
             a.top_logp[(uint64_t)r * K + place] = none ? -INFINITY : (key_value((uint32_t)(k >> 32)) - m) - ls;
         }
