@@ -592,6 +592,7 @@ lssm_status lssm_logprobs(lssm_ctx* ctx, const void* logits, const uint32_t* tar
     a.logp = logp; a.entropy = entropy; a.lse = lse; a.top_ids = top_ids; a.top_logp = top_logp;
     a.rows = d.rows; a.vocab = d.vocab; a.top_k = d.top_k; a.dtype = d.dtype;
     a.row_stride = d.row_stride ? d.row_stride : d.vocab;
+    a.sm_count = ctx->sm_count;
     LAUNCH("logprobs", launch_logprobs(a, ctx->stream));
 }
 

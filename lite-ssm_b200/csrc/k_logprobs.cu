@@ -20,8 +20,9 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
+constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32, LP_TOPS = 32 / LP_WARPS;
 constexpr int LP_GROUP = 4;          // 16-byte loads that a thread has on their way while it works on as many
+constexpr int LP_CTAS = 4;           // CTAs an SM holds
 constexpr int LP_CAND = 1024;        // candidates for the top entries that a CTA holds
 constexpr int LP_HITS = 256;         // chunks that may hold one
 constexpr int LP_CLUSTER_MAX = 8;
@@ -131,21 +132,34 @@ __device__ __forceinline__ float2 to_float2(uint32_t w, __nv_bfloat16) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
 
-// The largest of a chunk's elements; a NaN counts only where there is nothing else.
-__device__ __forceinline__ float chunk_max(uint4 c, __half) {
-    __half2 h[4];
-    memcpy(h, &c, 16);
-    const float2 f = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
-    return fmaxf(f.x, f.y);
+// The largest element of n chunks; a NaN counts only where there is nothing else.
+template <typename T, int n>
+__device__ __forceinline__ float chunks_max(const uint4 (&c)[n]) {
+    if constexpr (sizeof(T) == 4) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < n; ++i)
+            m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(c[i].x), __uint_as_float(c[i].y)),
+                               fmaxf(__uint_as_float(c[i].z), __uint_as_float(c[i].w))));
+        return m;
+    } else {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        T2 h[4 * n];
+        memcpy(h, c, sizeof(h));
+#pragma unroll
+        for (int w = 2 * n; w; w /= 2)
+#pragma unroll
+            for (int i = 0; i < w; ++i) h[i] = __hmax2(h[i], h[i + w]);
+        uint32_t b;
+        memcpy(&b, &h[0], 4);
+        const float2 f = to_float2(b, T());
+        return fmaxf(f.x, f.y);
+    }
 }
-__device__ __forceinline__ float chunk_max(uint4 c, __nv_bfloat16) {
-    __nv_bfloat162 h[4];
-    memcpy(h, &c, 16);
-    const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
-    return fmaxf(f.x, f.y);
-}
-__device__ __forceinline__ float chunk_max(uint4 c, float) {
-    return fmaxf(fmaxf(__uint_as_float(c.x), __uint_as_float(c.y)), fmaxf(__uint_as_float(c.z), __uint_as_float(c.w)));
+template <typename T>
+__device__ __forceinline__ float chunk_max(uint4 c, T) {
+    const uint4 one[1] = {c};
+    return chunks_max<T, 1>(one);
 }
 template <typename T>
 __device__ __forceinline__ void chunk_values(uint4 c, float (&v)[16 / sizeof(T)]) {
@@ -198,15 +212,19 @@ struct Sums {
         s2 = add2(s2, e);
         u2 = fma2(e, z, u2);
     }
-    __device__ __forceinline__ void chunk(uint4 c) {
-        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    // n chunks whose largest element is gm
+    template <int n>
+    __device__ __forceinline__ void chunks(const uint4 (&c)[n], float gm) {
+        follow(gm);
+        uint32_t w[4 * n];
+        memcpy(w, c, sizeof(w));
         if constexpr (std::is_same<T, __half>::value) {
             const uint64_t l2 = pack2(LOG2E, LOG2E), r2 = pack2(-refL, -refL);
             if (ref > -60000.0f) {
                 // -inf becomes the lowest finite value: its exponential is 0 too, but times z it is 0, not NaN
                 const __half2 low = __half2half2(__ushort_as_half(0xFBFF));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 4 * n; ++i) {
                     __half2 h;
                     memcpy(&h, &w[i], 4);
                     const float2 f = __half22float2(__hmax2_nan(h, low));
@@ -215,7 +233,7 @@ struct Sums {
             } else {
                 // nothing but -inf and values near the lowest so far: they have to be told apart
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 4 * n; ++i) {
                     const float2 f = to_float2(w[i], T());
                     const float2 z = unpack2(fma2(pack2(f.x, f.y), l2, r2));
                     add(pack2(max_or_nan(z.x, -300.0f), max_or_nan(z.y, -300.0f)));
@@ -223,17 +241,14 @@ struct Sums {
             }
         } else {
             const float r = ref > -INFINITY ? ref : 0.0f;
-            if constexpr (sizeof(T) == 4) {
+            const uint64_t l2 = pack2(LOG2E, LOG2E), zero = pack2(-0.0f, -0.0f), r2 = pack2(-r, -r);
 #pragma unroll
-                for (int i = 0; i < 4; i += 2)
-                    add(pack2(max_or_nan((__uint_as_float(w[i]) - r) * LOG2E, -300.0f),
-                              max_or_nan((__uint_as_float(w[i + 1]) - r) * LOG2E, -300.0f)));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 f = to_float2(w[i], T());
-                    add(pack2(max_or_nan((f.x - r) * LOG2E, -300.0f), max_or_nan((f.y - r) * LOG2E, -300.0f)));
-                }
+            for (int i = 0; i < 4 * n; i += sizeof(T) / 2) {
+                float2 f;
+                if constexpr (sizeof(T) == 4) f = make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1]));
+                else f = to_float2(w[i], T());
+                const float2 z = unpack2(fma2(add2(pack2(f.x, f.y), r2), l2, zero));
+                add(pack2(max_or_nan(z.x, -300.0f), max_or_nan(z.y, -300.0f)));
             }
         }
     }
@@ -248,7 +263,7 @@ struct LpShared {
     float m[LP_CLUSTER_MAX], s[LP_CLUSTER_MAX], u[LP_CLUSTER_MAX];
     uint64_t list[LP_CLUSTER_MAX][LSSM_TOP_K_MAX];
     float red[2][LP_WARPS];
-    alignas(16) uint32_t maxima[LP_WARPS * 4];        // the four largest thread maxima of every warp (order_key)
+    alignas(16) uint32_t maxima[32];                  // the LP_TOPS largest thread maxima of every warp (order_key)
     uint32_t count, nhits, nsel, bound, wsum[LP_WARPS];
     uint64_t wbest[LP_WARPS];
     uint8_t sel[LP_THREADS];
@@ -273,10 +288,11 @@ __device__ __forceinline__ void find_bound(uint32_t K, LpShared& sh) {
 //
 // sh.bound is a value that at least K entries reach. Only threads whose maximum reaches it can hold one of the
 // top K, so only their chunks (about K / 256 of the slice, still in L2) are read again, and of those that reach
-// it the elements. What reaches the bound is ranked by value and index.
+// it the elements. What reaches the bound is ranked by value and index. Thread t has chunks c0 + t, + LP_THREADS,
+// ... (`dealt`: lane l of warp w has chunk c0 + l * LP_WARPS + w).
 template <typename T>
 __device__ __forceinline__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t c1, uint32_t tkey, uint32_t K, LpShared& sh,
-                                        uint64_t* list) {
+                                        bool dealt, uint64_t* list) {
     constexpr int VEC = 16 / sizeof(T);
     const uint32_t tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const uint32_t bound = sh.bound;
@@ -285,7 +301,7 @@ __device__ __forceinline__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t
     uint32_t at = 0;
     if (lane == 0 && votes) at = atomicAdd(&sh.nsel, __popc(votes));
     at = __shfl_sync(FULL, at, 0) + __popc(votes & ((1u << lane) - 1));
-    if (chosen) sh.sel[at] = (uint8_t)tid;
+    if (chosen) sh.sel[at] = (uint8_t)(dealt ? lane * LP_WARPS + wid : tid);
     __syncthreads();
     const uint32_t nsel = sh.nsel;
     const float bv = key_value(bound);
@@ -293,21 +309,31 @@ __device__ __forceinline__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t
     auto collect = [&](bool ties) {
         // a warp takes four chosen threads at a time, a lane one of their chunks
         for (uint32_t i = wid * 4; i < nsel; i += LP_WARPS * 4)
-            for (uint32_t k = lane * LP_THREADS; c0 + k < c1; k += 32 * LP_THREADS) {
+            for (uint32_t k0 = 0; c0 + k0 < c1; k0 += 32 * LP_THREADS) {
+                const uint32_t k = k0 + lane * LP_THREADS;
                 uint4 w[4];
-                uint32_t c[4];
+                uint32_t c[4], m[4];
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    c[g] = i + g < nsel ? c0 + k + sh.sel[i + g] : c1;
+                    c[g] = i + g < nsel ? min(c1, c0 + k + sh.sel[i + g]) : c1;
                     if (c[g] < c1) w[g] = row.chunk(c[g]);
                 }
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    if (c[g] >= c1) continue;
-                    const float cm = chunk_max(w[g], T());
-                    if (ties ? cm < bv : cm <= bv) continue;
-                    const uint32_t p = atomicAdd(&sh.nhits, 1u);
-                    if (p < LP_HITS) { sh.hit[p] = w[g]; sh.hit_at[p] = c[g]; }
+                    const float cm = c[g] < c1 ? chunk_max(w[g], T()) : -INFINITY;
+                    const bool is = c[g] < c1 && !(ties ? cm < bv : cm <= bv);
+                    m[g] = __ballot_sync(FULL, is);
+                }
+                const uint32_t total = __popc(m[0]) + __popc(m[1]) + __popc(m[2]) + __popc(m[3]);
+                if (!total) continue;
+                uint32_t p = 0;
+                if (lane == 0) p = atomicAdd(&sh.nhits, total);
+                p = __shfl_sync(FULL, p, 0);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const uint32_t q = p + __popc(m[g] & ((1u << lane) - 1));
+                    if ((m[g] >> lane & 1) && q < LP_HITS) { sh.hit[q] = w[g]; sh.hit_at[q] = c[g]; }
+                    p += __popc(m[g]);
                 }
             }
         __syncthreads();
@@ -411,9 +437,9 @@ __device__ __forceinline__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t
     if (tid >= n && tid < LSSM_TOP_K_MAX) list[tid] = 0;
 }
 
-// One CTA, or a cluster of them over slices of the vocabulary, per row; one pass over the logits.
+// One CTA, or a cluster of nc over slices of the vocabulary, per row; one pass over the logits.
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(LogprobsArgs a, uint32_t nc) {
+__global__ void __launch_bounds__(LP_THREADS, LP_CTAS) k_logprobs(LogprobsArgs a, uint32_t nc) {
     __shared__ LpShared sh;
     const uint32_t tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const uint32_t r = blockIdx.x / nc, part = blockIdx.x % nc;
@@ -429,14 +455,9 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(LogprobsArgs a, uint
     // loaded before this one is worked on, and one by one what is left of the slice's ends.
     const uint32_t inner = row.inner(), outer = min(c1, row.outer());
     constexpr uint32_t STRIDE = LP_THREADS * LP_GROUP;
-    uint32_t c = c0 + tid;
-    auto single = [&](uint32_t k) {
-        const uint4 w = row.chunk(k);
-        const float gm = chunk_max(w, T());
-        tmax = fmaxf(tmax, gm);
-        sum.follow(gm);
-        sum.chunk(w);
-    };
+    // a slice with less than a chunk a thread is dealt to the warps in turn, so that all of them have maxima
+    const bool dealt = c1 - c0 < LP_THREADS;
+    uint32_t c = c0 + (dealt ? lane * LP_WARPS + wid : tid);
     const bool head = c < inner;
     if (head) c += LP_THREADS;
     uint32_t groups = c < outer ? (outer - c + LP_THREADS - 1) / LP_THREADS / LP_GROUP : 0;
@@ -447,18 +468,26 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(LogprobsArgs a, uint
         at += STRIDE;
     };
     auto work = [&](const uint4 (&d)[LP_GROUP]) {
-        float gm = chunk_max(d[0], T());
-#pragma unroll
-        for (int g = 1; g < LP_GROUP; ++g) gm = fmaxf(gm, chunk_max(d[g], T()));
+        const float gm = chunks_max<T>(d);
         tmax = fmaxf(tmax, gm);
-        sum.follow(gm);
-#pragma unroll
-        for (int g = 0; g < LP_GROUP; ++g) sum.chunk(d[g]);
+        sum.chunks(d, gm);
+    };
+    auto single = [&](uint4 d) {
+        const uint4 one[1] = {d};
+        const float gm = chunks_max<T>(one);
+        tmax = fmaxf(tmax, gm);
+        sum.chunks(one, gm);
     };
     uint4 w[LP_GROUP], next[LP_GROUP];
     if (groups) load(w);
-    if (head) single(c - LP_THREADS);
-    for (uint32_t k = c + groups * STRIDE; k < c1; k += LP_THREADS) single(k);
+    const uint32_t rest = c + groups * STRIDE;   // at most LP_GROUP chunks
+#pragma unroll
+    for (int g = 0; g < LP_GROUP; ++g)
+        if (rest + g * LP_THREADS < c1) next[g] = row.chunk(rest + g * LP_THREADS);
+    if (head) single(row.chunk(c - LP_THREADS));
+#pragma unroll
+    for (int g = 0; g < LP_GROUP; ++g)
+        if (rest + g * LP_THREADS < c1) single(next[g]);
     while (groups) {
         if (--groups) load(next);
         work(w);
@@ -466,13 +495,15 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(LogprobsArgs a, uint
         if (--groups) load(w);
         work(next);
     }
+    float xt = 0.0f;
+    if (target < a.vocab) xt = load_one(row.x + target);
     // the largest thread maxima of every warp, the CTA's maximum, and the sums against it
     const uint32_t tkey = order_key(tmax), K = a.top_k;
     uint32_t mine = tkey;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < LP_TOPS; ++q) {
         const uint32_t top = __reduce_max_sync(FULL, mine);
-        if (lane == 0) sh.maxima[wid * 4 + q] = top;
+        if (lane == 0) sh.maxima[wid * LP_TOPS + q] = top;
         if ((int)lane == __ffs(__ballot_sync(FULL, mine == top)) - 1) mine = 0;
     }
     if (tid == 0) { sh.count = 0; sh.nhits = 0; sh.nsel = 0; }
@@ -489,7 +520,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(LogprobsArgs a, uint
     s = u = 0.0f;
 #pragma unroll
     for (int w = 0; w < LP_WARPS; ++w) { s += sh.red[0][w]; u += sh.red[1][w]; }
-    if (K) cta_top(row, c0, c1, tkey, K, sh, sh.list[part]);
+    if (K) cta_top(row, c0, c1, tkey, K, sh, dealt, sh.list[part]);
     __syncthreads();
     if (nc > 1) {
         // the slices' sums and lists meet in the first CTA of the cluster, whose CTAs all run by now
@@ -521,24 +552,25 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(LogprobsArgs a, uint
         if (a.logp) {
             float v = 0.0f;
             if (target != LSSM_NO_TOKEN)
-                v = target >= a.vocab ? __int_as_float(0x7FC00000) : none ? -INFINITY : (load_one(row.x + target) - m) - ls;
+                v = target >= a.vocab ? __int_as_float(0x7FC00000) : none ? -INFINITY : (xt - m) - ls;
             a.logp[r] = v;
         }
     }
-    if (wid < nc && lane < K) {
-        // entry `lane` of list `wid`; its place: the entries before it, in its own list and in the others
-        const uint64_t k = sh.list[wid][lane];
+    for (uint32_t l = wid; l < nc && lane < K; l += LP_WARPS) {
+        // entry `lane` of list `l`; its place: the entries before it, in its own list and in the others
+        const uint64_t k = sh.list[l][lane];
         uint32_t place = lane;
         if (nc > 1) {
+            uint32_t lo[LP_CLUSTER_MAX] = {};
 #pragma unroll
-            for (uint32_t p = 0; p < LP_CLUSTER_MAX; ++p) {
-                if (p >= nc || p == wid) continue;
-                uint32_t lo = 0;
+            for (uint32_t step = 16; step; step >>= 1)
 #pragma unroll
-                for (uint32_t step = 16; step; step >>= 1)
-                    if (lo + step <= K && sh.list[p][lo + step - 1] > k) lo += step;
-                if (lo < K && sh.list[p][lo] > k) ++lo;
-                place += lo;
+                for (uint32_t q = 0; q < LP_CLUSTER_MAX; ++q)
+                    if (lo[q] + step <= K && sh.list[q][lo[q] + step - 1] > k) lo[q] += step;
+#pragma unroll
+            for (uint32_t q = 0; q < LP_CLUSTER_MAX; ++q) {
+                if (lo[q] < K && sh.list[q][lo[q]] > k) ++lo[q];
+                if (q < nc && q != l) place += lo[q];
             }
         }
         if (k && place < K) {
@@ -548,34 +580,116 @@ __global__ void __launch_bounds__(LP_THREADS, 4) k_logprobs(LogprobsArgs a, uint
     }
 }
 
-__global__ void __launch_bounds__(LP_THREADS) k_logprobs_grad(LogprobsGradArgs a) {
-    const uint32_t r = blockIdx.x, V = a.vocab;
-    const uint64_t xb = (uint64_t)r * a.row_stride, gb = (uint64_t)r * a.grad_stride;
-    const float lse = a.lse[r], H = a.g_entropy ? a.entropy[r] : 0.0f;
-    const uint32_t t = a.targets ? a.targets[r] : LSSM_NO_TOKEN;
-    const bool none = lse == -INFINITY, given = t != LSSM_NO_TOKEN;
-    float g = a.g_logp && given ? a.g_logp[r] : 0.0f;
-    const float h = a.g_entropy ? a.g_entropy[r] : 0.0f;
-    if (given && t >= V) g = __int_as_float(0x7FC00000);
-    for (uint32_t i = threadIdx.x; i < V; i += LP_THREADS) {
-        float d = 0.0f;
-        if (!none) {
-            const float lp = load_any(a.logits, xb + i, a.dtype) - lse, p = expf(lp);
-            d = (i == t ? g : 0.0f) - g * p;
-            if (a.g_entropy && p != 0.0f) d -= h * p * (lp + H);
-        }
-        store_any(a.dlogits, gb + i, a.grad_dtype, d);
+// What a row's elements have in common, for d_j = g [j = t] - p_j (g + h (log p_j + H)).
+struct GradRow {
+    float lse, g, h, H;
+    uint32_t t;
+    bool none;
+    __device__ GradRow(const LogprobsGradArgs& a, uint32_t r) {
+        lse = a.lse[r];
+        t = a.targets ? a.targets[r] : LSSM_NO_TOKEN;
+        h = a.g_entropy ? a.g_entropy[r] : 0.0f;
+        H = a.g_entropy ? a.entropy[r] : 0.0f;
+        none = lse == -INFINITY;
+        g = a.g_logp && t != LSSM_NO_TOKEN ? a.g_logp[r] : 0.0f;
+        if (t != LSSM_NO_TOKEN && t >= a.vocab) g = __int_as_float(0x7FC00000);
     }
+    template <bool ENTROPY>
+    __device__ __forceinline__ float operator()(float x, uint32_t j) const {
+        const float lp = x - lse, p = ex2(lp * LOG2E);
+        // p = 0 ends a masked entry: its log p may be -inf
+        const float d = ENTROPY ? (p == 0.0f ? 0.0f : -p * fmaf(h, lp + H, g)) : -p * g;
+        return none ? 0.0f : j == t ? d + g : d;
+    }
+};
+
+template <typename G> __device__ __forceinline__ void store_one(G* p, float v);
+template <> __device__ __forceinline__ void store_one(__half* p, float v) { *p = __float2half_rn(v); }
+template <> __device__ __forceinline__ void store_one(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
+
+// n consecutive elements, as wide as their address allows.
+template <typename G, int n>
+__device__ __forceinline__ void store_some(G* p, const float (&v)[n]) {
+    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && n * sizeof(G) >= 16) {
+        uint32_t w[n * sizeof(G) / 4];
+#pragma unroll
+        for (int i = 0; i < (int)(n * sizeof(G) / 4); ++i) {
+            if constexpr (sizeof(G) == 4) w[i] = __float_as_uint(v[i]);
+            else if constexpr (std::is_same<G, __half>::value) { const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]); memcpy(&w[i], &h, 4); }
+            else { const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]); memcpy(&w[i], &h, 4); }
+        }
+#pragma unroll
+        for (int i = 0; i < (int)(n * sizeof(G) / 16); ++i)
+            __stcs(reinterpret_cast<uint4*>(p) + i, make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < n; ++i) store_one(p + i, v[i]);
+    }
+}
+
+// Elementwise: one read, one write. A CTA takes GRAD_CHUNKS chunks a thread of one row (a chunk is 16 bytes of
+// logits); all of them are loaded before the first is worked on.
+constexpr int GRAD_CHUNKS = 4;
+template <typename T, typename G, bool ENTROPY>
+__global__ void __launch_bounds__(LP_THREADS) k_logprobs_grad(LogprobsGradArgs a, uint32_t parts) {
+    constexpr int VEC = 16 / sizeof(T);
+    const uint32_t r = blockIdx.x / parts, part = blockIdx.x % parts;
+    const Row<T> row(a.logits, (uint64_t)r * a.row_stride, a.vocab);
+    G* out = static_cast<G*>(a.dlogits) + (uint64_t)r * a.grad_stride;
+    const uint32_t c0 = part * (LP_THREADS * GRAD_CHUNKS) + threadIdx.x;
+    uint4 w[GRAD_CHUNKS];
+#pragma unroll
+    for (int i = 0; i < GRAD_CHUNKS; ++i) {
+        const uint32_t c = c0 + i * LP_THREADS;
+        if (c >= row.inner() && c < row.outer()) w[i] = __ldcs(row.base() + c);
+    }
+    const GradRow grad(a, r);
+#pragma unroll
+    for (int i = 0; i < GRAD_CHUNKS; ++i) {
+        const uint32_t c = c0 + i * LP_THREADS;
+        if (c >= row.chunks) break;
+        const int64_t e = row.index(c);
+        if (c >= row.inner() && c < row.outer()) {
+            float x[VEC], d[VEC];
+            chunk_values<T>(w[i], x);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) d[j] = grad.template operator()<ENTROPY>(x[j], (uint32_t)e + j);
+            store_some<G, VEC>(out + e, d);
+        } else {
+            for (int j = 0; j < VEC; ++j)
+                if (e + j >= 0 && e + j < (int64_t)row.V)
+                    store_one(out + e + j, grad.template operator()<ENTROPY>(load_one(row.x + e + j), (uint32_t)(e + j)));
+        }
+    }
+}
+
+template <typename T, typename G>
+cudaError_t launch_grad(const LogprobsGradArgs& a, cudaStream_t s) {
+    constexpr uint32_t VEC = 16 / sizeof(T), SPAN = LP_THREADS * GRAD_CHUNKS;
+    // one chunk more than the elements fill: a row may begin inside one
+    const uint64_t parts = ((uint64_t)a.vocab + 2 * VEC - 2) / VEC / SPAN + 1, grid = parts * a.rows;
+    if (grid > 0x7FFFFFFFu) return cudaErrorInvalidValue;
+    if (a.g_entropy) k_logprobs_grad<T, G, true><<<(unsigned)grid, LP_THREADS, 0, s>>>(a, (uint32_t)parts);
+    else k_logprobs_grad<T, G, false><<<(unsigned)grid, LP_THREADS, 0, s>>>(a, (uint32_t)parts);
+    return cudaGetLastError();
+}
+template <typename T>
+cudaError_t launch_grad_of(const LogprobsGradArgs& a, cudaStream_t s) {
+    if (a.grad_dtype == LSSM_DT_F16) return launch_grad<T, __half>(a, s);
+    if (a.grad_dtype == LSSM_DT_BF16) return launch_grad<T, __nv_bfloat16>(a, s);
+    return launch_grad<T, float>(a, s);
 }
 
 }  // namespace
 
 cudaError_t launch_logprobs(const LogprobsArgs& a, cudaStream_t s) {
     if (!a.rows) return cudaSuccess;
-    // Few rows: a cluster of CTAs a row, until every SM has two CTAs or a thread less than one chunk.
+    // A few long rows: a cluster of CTAs a row. A cluster costs its launch and its join: slices below 32 K entries
+    // and more than about two CTAs an SM lose by it (256000 fp16 entries, top 5: 1 row 20.1 us with one CTA, 9.2
+    // with 8; 64 rows 28.0 / 18.5 / 14.4 / 16.5 with 1 / 2 / 4 / 8; 50288 entries, 128 rows 10.1 / 10.3 / 12.5).
     uint32_t nc = 1;
-    while (nc < LP_CLUSTER_MAX && (uint64_t)a.rows * nc < 296 && a.vocab / (8 * LP_THREADS * nc) >= 1) nc *= 2;
-    if ((uint64_t)a.rows * nc > 0x7FFFFFFFull) nc = 1;
+    while (nc < LP_CLUSTER_MAX && (uint64_t)a.rows * nc * 2 <= 400 && a.vocab / (nc * 2) >= 32000) nc *= 2;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim = {nc, 1, 1};
@@ -595,8 +709,9 @@ cudaError_t launch_logprobs(const LogprobsArgs& a, cudaStream_t s) {
 
 cudaError_t launch_logprobs_grad(const LogprobsGradArgs& a, cudaStream_t s) {
     if (!a.rows) return cudaSuccess;
-    k_logprobs_grad<<<a.rows, LP_THREADS, 0, s>>>(a);
-    return cudaGetLastError();
+    if (a.dtype == LSSM_DT_F16) return launch_grad_of<__half>(a, s);
+    if (a.dtype == LSSM_DT_BF16) return launch_grad_of<__nv_bfloat16>(a, s);
+    return launch_grad_of<float>(a, s);
 }
 
 }  // namespace lssm

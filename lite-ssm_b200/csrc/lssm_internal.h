@@ -146,6 +146,7 @@ struct LogprobsArgs {
     float* logp; float* entropy; float* lse; uint32_t* top_ids; float* top_logp;
     uint32_t rows, vocab, top_k, dtype;
     uint64_t row_stride;
+    int sm_count;
 };
 cudaError_t launch_logprobs(const LogprobsArgs& a, cudaStream_t s);
 struct LogprobsGradArgs {
