@@ -608,28 +608,29 @@ template <> __device__ __forceinline__ void store_one(__half* p, float v) { *p =
 template <> __device__ __forceinline__ void store_one(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
 
-// n consecutive elements, as wide as their address allows.
+// The elements of one chunk in stores of 16 bytes (8 where they make no more), whose address has to allow it.
 template <typename G, int n>
-__device__ __forceinline__ void store_some(G* p, const float (&v)[n]) {
-    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && n * sizeof(G) >= 16) {
-        uint32_t w[n * sizeof(G) / 4];
+constexpr uint32_t STORE = n * sizeof(G) >= 16 ? 16 : 8;
+template <typename G, int n>
+__device__ __forceinline__ void store_chunk(G* p, const float (&v)[n]) {
+    uint32_t w[n * sizeof(G) / 4];
 #pragma unroll
-        for (int i = 0; i < (int)(n * sizeof(G) / 4); ++i) {
-            if constexpr (sizeof(G) == 4) w[i] = __float_as_uint(v[i]);
-            else if constexpr (std::is_same<G, __half>::value) { const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]); memcpy(&w[i], &h, 4); }
-            else { const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]); memcpy(&w[i], &h, 4); }
-        }
+    for (int i = 0; i < (int)(n * sizeof(G) / 4); ++i) {
+        if constexpr (sizeof(G) == 4) w[i] = __float_as_uint(v[i]);
+        else if constexpr (std::is_same<G, __half>::value) { const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]); memcpy(&w[i], &h, 4); }
+        else { const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]); memcpy(&w[i], &h, 4); }
+    }
+    if constexpr (STORE<G, n> == 8) __stcs(reinterpret_cast<uint2*>(p), make_uint2(w[0], w[1]));
+    else
 #pragma unroll
         for (int i = 0; i < (int)(n * sizeof(G) / 16); ++i)
             __stcs(reinterpret_cast<uint4*>(p) + i, make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
-    } else {
-#pragma unroll
-        for (int i = 0; i < n; ++i) store_one(p + i, v[i]);
-    }
 }
 
 // Elementwise: one read, one write. A CTA takes GRAD_CHUNKS chunks a thread of one row (a chunk is 16 bytes of
-// logits); all of them are loaded before the first is worked on.
+// logits); all of them are loaded before the first is worked on. Where the chunks' places in the output are not
+// aligned for wide stores, a warp exchanges its 32 chunks through shared memory, so that a store instruction
+// writes 32 neighbours.
 constexpr int GRAD_CHUNKS = 4;
 template <typename T, typename G, bool ENTROPY>
 __global__ void __launch_bounds__(LP_THREADS) k_logprobs_grad(LogprobsGradArgs a, uint32_t parts) {
@@ -645,18 +646,32 @@ __global__ void __launch_bounds__(LP_THREADS) k_logprobs_grad(LogprobsGradArgs a
         if (c >= row.inner() && c < row.outer()) w[i] = __ldcs(row.base() + c);
     }
     const GradRow grad(a, r);
+    __shared__ float swap[LP_WARPS][32 * (VEC + 1)];   // a chunk to VEC + 1 words: no bank twice
+    const uint32_t lane = threadIdx.x & 31;
+    const bool wide = reinterpret_cast<uintptr_t>(out + row.index(row.inner())) % STORE<G, VEC> == 0;
 #pragma unroll
     for (int i = 0; i < GRAD_CHUNKS; ++i) {
         const uint32_t c = c0 + i * LP_THREADS;
-        if (c >= row.chunks) break;
+        const bool inside = c >= row.inner() && c < row.outer();
         const int64_t e = row.index(c);
-        if (c >= row.inner() && c < row.outer()) {
-            float x[VEC], d[VEC];
+        float d[VEC];
+        if (inside) {
+            float x[VEC];
             chunk_values<T>(w[i], x);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) d[j] = grad.template operator()<ENTROPY>(x[j], (uint32_t)e + j);
-            store_some<G, VEC>(out + e, d);
-        } else {
+        }
+        if (wide && inside) {
+            store_chunk<G, VEC>(out + e, d);
+        } else if (!wide && __all_sync(FULL, inside)) {
+            float* mine = swap[threadIdx.x / 32];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) mine[lane * (VEC + 1) + j] = d[j];
+            __syncwarp();
+#pragma unroll
+            for (uint32_t q = lane; q < 32 * VEC; q += 32) store_one(out + e - lane * VEC + q, mine[q / VEC * (VEC + 1) + q % VEC]);
+            __syncwarp();
+        } else if (c < row.chunks) {
             for (int j = 0; j < VEC; ++j)
                 if (e + j >= 0 && e + j < (int64_t)row.V)
                     store_one(out + e + j, grad.template operator()<ENTROPY>(load_one(row.x + e + j), (uint32_t)(e + j)));
