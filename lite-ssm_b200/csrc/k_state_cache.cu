@@ -28,20 +28,62 @@ __device__ __forceinline__ float token_dt(float raw, float lo, float hi) {
     return fminf(fmaxf(raw > 20.0f ? raw : log1pf(expf(raw)), lo), hi);
 }
 
-// The nearest code to v / scale. The product with the reciprocal may land on the wrong side of a
-// half step; the remainder v - q * scale, exact in one fma, decides.
-__device__ __forceinline__ int nearest_code(float v, float scale, float inv, float Q) {
-    if (!(scale > 0.0f)) return 0;   // zero row, or NaN scale
-    float q = fminf(fmaxf(rintf(v * inv), -Q), Q);
-    const float r = fmaf(-q, scale, v), half = 0.5f * scale;
-    if (fabsf(r) > half) q += r > 0.0f ? 1.0f : -1.0f;
-    else if (fabsf(r) == half && ((int)q & 1)) q += r > 0.0f ? 1.0f : -1.0f;
-    return (int)fminf(fmaxf(q, -Q), Q);
+// A row's scale and what its codes are computed with.
+struct RowQuant {
+    float scale, inv, half;   // half: what a remainder may be at most
+    bool sound;               // no NaN, no infinity
+    // amax: the row's largest magnitude, NaN or infinite where an element is
+    __device__ __forceinline__ RowQuant(float amax, float Q) {
+        scale = __fdiv_rn(amax, Q);
+        sound = amax < INFINITY;
+        if (!sound) scale = __int_as_float(0x7FC00000);
+        else if (scale < kTiny) scale = 0.0f;
+        inv = scale > 0.0f ? __frcp_rn(scale) : 0.0f;
+        half = scale > 0.0f ? 0.5f * scale : INFINITY;
+    }
+};
+// Codes of four elements as whole numbers in the low bits of the results. Added to 1.5 * 2^23, v / scale is rounded
+// to a whole number, ties to even, but the reciprocal may have carried it over a half step. The remainder
+// v - q * scale, exact in one fma, tells: only where it is half a step or more (about once in a million) is the
+// code looked at again.
+__device__ __forceinline__ void quantise4(const float (&v)[4], const RowQuant& z, uint32_t (&c)[4]) {
+    constexpr float MAGIC = 12582912.0f;
+    float worst = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float m = fmaf(v[i], z.inv, MAGIC);
+        c[i] = __float_as_uint(m);
+        worst = fmaxf(worst, fabsf(fmaf(MAGIC - m, z.scale, v[i])));
+    }
+    if (worst >= z.half) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float q = __uint_as_float(c[i]) - MAGIC, r = fmaf(-q, z.scale, v[i]);
+            if (fabsf(r) > z.half || (fabsf(r) == z.half && (c[i] & 1))) c[i] += r > 0.0f ? 1 : -1;
+        }
+    }
 }
-__device__ __forceinline__ float row_scale(float amax, float Q) {
-    const float s = __fdiv_rn(amax, Q);
-    if (!(amax < INFINITY)) return __int_as_float(0x7FC00000);
-    return s < kTiny ? 0.0f : s;
+
+template <typename Code>
+__device__ __forceinline__ Code quantise1(float v, const RowQuant& z) {
+    const float four[4] = {v, 0.0f, 0.0f, 0.0f};
+    uint32_t c[4];
+    quantise4(four, z, c);
+    return z.sound ? (Code)c[0] : (Code)0;
+}
+// four codes, side by side
+__device__ __forceinline__ uint32_t pack_codes8(const uint32_t (&c)[4]) {
+    return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+}
+__device__ __forceinline__ uint2 pack_codes16(const uint32_t (&c)[4]) {
+    return make_uint2(__byte_perm(c[0], c[1], 0x5410), __byte_perm(c[2], c[3], 0x5410));
+}
+template <typename Code>
+__device__ __forceinline__ void store_codes4(Code* to, const float (&v)[4], const RowQuant& z) {
+    uint32_t c[4];
+    quantise4(v, z, c);
+    if constexpr (sizeof(Code) == 1) *reinterpret_cast<uint32_t*>(to) = z.sound ? pack_codes8(c) : 0u;
+    else *reinterpret_cast<uint2*>(to) = z.sound ? pack_codes16(c) : make_uint2(0u, 0u);
 }
 // max|.| that keeps NaN
 __device__ __forceinline__ float max_nan(float a, float b) { return a != a || b != b ? __int_as_float(0x7FC00000) : fmaxf(a, b); }
@@ -141,13 +183,13 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_cached(StateCacheArgs a) {
                 a.win_x[((uint64_t)b * a.W + n) * xrow + o] = xn[p];
             }
             if (fold) {
-                const float scale = row_scale(warp_max_nan(amax), Q), inv = scale > 0.0f ? 1.0f / scale : 0.0f;
+                const RowQuant z(warp_max_nan(amax), Q);
                 for (uint32_t i0 = 0; i0 < a.N; i0 += 32) {
                     const uint32_t i = i0 + lane;
                     const float v = state(i, i < a.N);
-                    if (i < a.N) row[i] = (Code)nearest_code(v, scale, inv, Q);
+                    if (i < a.N) row[i] = quantise1<Code>(v, z);
                 }
-                if (lane == 0) a.scales[bh * a.P + p] = scale;
+                if (lane == 0) a.scales[bh * a.P + p] = z.scale;
             }
         }
     }
@@ -163,7 +205,8 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_cached(StateCacheArgs a) {
 // ---------------------------------------------------------------------------
 //  N = 128, P a multiple of 16: tensor-core kernel
 // ---------------------------------------------------------------------------
-// A CTA per (sequence, head); a warp takes 16 rows of the state at a time. With m16n8k16 (f16 in, f32 out), lane
+// A CTA takes `heads` heads of one group and sequence; a warp 16 rows of a head's state at a time. With m16n8k16
+// (f16 in, f32 out), lane
 // (g, t) = (lane / 4, lane % 4), and an order of k that lets a lane load its codes as they lie:
 //   S_q C       A = codes (exact in f16: 8 bits as they are, 16 bits as 256 * high + low), B = C in every column
 //   C . B_j     A = the window's B rows, B = C in every column (one warp; 16 tokens an instruction)
@@ -171,14 +214,8 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_cached(StateCacheArgs a) {
 //               the largest at 2^14, B = the window's B; a lane gets the elements whose codes it holds.
 // A code is converted, multiplied and added in about one instruction for 30 elements, so the step is bound by the
 // codes' bytes and the latency of a short CTA.
-constexpr int TC_THREADS = 128, TC_N = 128;
-// Element order: lane t's word q (4 codes) is elements k0 .. k0 + 3. Steps load 16 bytes a lane; loads write 16 bytes
-// of fp32 a lane, with 4 neighbours in 4 lanes.
-template <typename Code, int MODE>
-__device__ __forceinline__ constexpr int tc_k0(int q, int t) {
-    return MODE == 1 ? 16 * q + 4 * t : sizeof(Code) == 1 ? 64 * (q / 4) + 16 * t + 4 * (q % 4) : 32 * (q / 2) + 8 * t + 4 * (q % 2);
-}
-
+constexpr int TC_THREADS = 256, TC_WARPS = TC_THREADS / 32, TC_N = 128, TC_HEADS = 4;
+constexpr uint32_t TC_ROWS = 256;   // rows of 8-bit codes a CTA holds (32 KB)
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -191,79 +228,25 @@ __device__ __forceinline__ uint32_t bytes_h2(uint32_t w, uint32_t sel, float off
     return h2_bits(__hsub2(bits_h2(__byte_perm(w, 0x64646464u, sel)), __float2half2_rn(off)));
 }
 
-// The codes of one row that a lane holds: 8 words of 4.
-template <typename Code>
-struct RowCodes {
-    static constexpr int REGS = 8 * sizeof(Code);
-    uint32_t r[REGS];
-    template <int MODE>
-    __device__ __forceinline__ void load(const Code* row, int t) {
-        if constexpr (MODE == 1) {
+// Four codes as fp32.
+__device__ __forceinline__ void code_values_of(uint32_t c, float (&v)[4]) {
+    const uint32_t w = c ^ 0x80808080u;
+    const float2 a = __half22float2(bits_h2(bytes_h2(w, 0x4140, 1152.0f)));
+    const float2 b = __half22float2(bits_h2(bytes_h2(w, 0x4342, 1152.0f)));
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+}
+__device__ __forceinline__ void code_values_of(uint2 c, float (&v)[4]) {
+    // added to 1.5 * 2^23 a 16-bit number is a float's low bits
+    const uint32_t w[2] = {c.x ^ 0x80008000u, c.y ^ 0x80008000u};
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                if constexpr (sizeof(Code) == 1) r[q] = *reinterpret_cast<const uint32_t*>(row + tc_k0<Code, 1>(q, t));
-                else {
-                    const uint2 v = *reinterpret_cast<const uint2*>(row + tc_k0<Code, 1>(q, t));
-                    r[2 * q] = v.x; r[2 * q + 1] = v.y;
-                }
-            }
-        } else {
-            constexpr int PER = 16 / sizeof(Code);   // codes a load
-#pragma unroll
-            for (int i = 0; i < REGS / 4; ++i) {
-                const uint4 v = *reinterpret_cast<const uint4*>(row + tc_k0<Code, 0>(i * PER / 4, t));
-                r[4 * i] = v.x; r[4 * i + 1] = v.y; r[4 * i + 2] = v.z; r[4 * i + 3] = v.w;
-            }
-        }
-    }
-    __device__ __forceinline__ void store(Code* row, int t) const {
-        constexpr int PER = 16 / sizeof(Code);
-#pragma unroll
-        for (int i = 0; i < REGS / 4; ++i)
-            *reinterpret_cast<uint4*>(row + tc_k0<Code, 0>(i * PER / 4, t)) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-    }
-    // word q as fp32
-    __device__ __forceinline__ void values(int q, float (&v)[4]) const {
-        if constexpr (sizeof(Code) == 1) {
-            const uint32_t w = r[q] ^ 0x80808080u;
-            const float2 a = __half22float2(bits_h2(bytes_h2(w, 0x4140, 1152.0f)));
-            const float2 b = __half22float2(bits_h2(bytes_h2(w, 0x4342, 1152.0f)));
-            v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
-        } else {
-            v[0] = (float)(int16_t)(r[2 * q] & 0xFFFF); v[1] = (float)((int32_t)r[2 * q] >> 16);
-            v[2] = (float)(int16_t)(r[2 * q + 1] & 0xFFFF); v[3] = (float)((int32_t)r[2 * q + 1] >> 16);
-        }
-    }
-    __device__ __forceinline__ void set(int q, const int (&c)[4]) {
-        if constexpr (sizeof(Code) == 1)
-            r[q] = (c[0] & 0xFF) | (c[1] & 0xFF) << 8 | (c[2] & 0xFF) << 16 | (uint32_t)c[3] << 24;
-        else {
-            r[2 * q] = (c[0] & 0xFFFF) | (uint32_t)c[1] << 16;
-            r[2 * q + 1] = (c[2] & 0xFFFF) | (uint32_t)c[3] << 16;
-        }
-    }
-};
+    for (int i = 0; i < 4; ++i)
+        v[i] = __uint_as_float(__byte_perm(w[i / 2], 0x4B400000u, i & 1 ? 0x7632 : 0x7610)) - (12582912.0f + 32768.0f);
+}
 
-// acc[0], acc[2] += codes . C of rows g and g + 8
 template <typename Code>
-__device__ __forceinline__ void codes_dot_c(const RowCodes<Code>& u, const RowCodes<Code>& v, const uint32_t (&c)[16], float (&y)[2]) {
-    float lo[4] = {}, hi[4] = {};
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        if constexpr (sizeof(Code) == 1) {
-            const uint32_t a = u.r[q] ^ 0x80808080u, b = v.r[q] ^ 0x80808080u;
-            mma16816(lo, bytes_h2(a, 0x4140, 1152.0f), bytes_h2(b, 0x4140, 1152.0f), bytes_h2(a, 0x4342, 1152.0f),
-                     bytes_h2(b, 0x4342, 1152.0f), c[2 * q], c[2 * q + 1]);
-        } else {
-            const uint32_t a0 = u.r[2 * q], a1 = u.r[2 * q + 1], b0 = v.r[2 * q], b1 = v.r[2 * q + 1];
-            mma16816(lo, bytes_h2(a0, 0x4240, 1024.0f), bytes_h2(b0, 0x4240, 1024.0f), bytes_h2(a1, 0x4240, 1024.0f),
-                     bytes_h2(b1, 0x4240, 1024.0f), c[2 * q], c[2 * q + 1]);
-            mma16816(hi, bytes_h2(a0 ^ 0x80008000u, 0x4341, 1152.0f), bytes_h2(b0 ^ 0x80008000u, 0x4341, 1152.0f),
-                     bytes_h2(a1 ^ 0x80008000u, 0x4341, 1152.0f), bytes_h2(b1 ^ 0x80008000u, 0x4341, 1152.0f), c[2 * q], c[2 * q + 1]);
-        }
-    }
-    y[0] = sizeof(Code) == 1 ? lo[0] : fmaf(256.0f, hi[0], lo[0]);
-    y[1] = sizeof(Code) == 1 ? lo[2] : fmaf(256.0f, hi[2], lo[2]);
+__device__ __forceinline__ void code_values(const uint8_t* at, float (&v)[4]) {
+    if constexpr (sizeof(Code) == 1) code_values_of(*reinterpret_cast<const uint32_t*>(at), v);
+    else code_values_of(*reinterpret_cast<const uint2*>(at), v);
 }
 
 __device__ __forceinline__ float max_keep_nan(float a, float b) {
@@ -271,185 +254,275 @@ __device__ __forceinline__ float max_keep_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
+__device__ __forceinline__ void copy_async16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+// Two f16 terms of (x0, x1): 22 bits together.
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t* hi, uint32_t* lo) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    const float2 f = __half22float2(h);
+    *hi = h2_bits(h);
+    *lo = h2_bits(__floats2half2_rn(x0 - f.x, x1 - f.y));
+}
+// A power of two that brings the largest of the warp's values to 2^14, and its inverse. Values that are not finite
+// set no scale.
+struct Pow2 {
+    float up, down;
+    template <int n>
+    __device__ __forceinline__ Pow2(const float (&v)[n]) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const uint32_t bits = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+            if (bits < 0x7F800000u) top = max(top, bits);
+        }
+        const uint32_t eb = max(__reduce_max_sync(0xffffffffu, top) >> 23, 15u);
+        up = __uint_as_float(min(268u - eb, 254u) << 23);
+        down = __uint_as_float((eb - 14u) << 23);
+    }
+};
+
+// Shared memory of a CTA: the heads' codes (rows of TC_N, their 16-byte pieces exchanged by row so that neither
+// 16-byte nor 4-byte reads of 8 rows meet in a bank), the window's x (a row a token) and B, the pair layout of B.
+template <typename Code, int KB>
+struct TcShared {
+    static constexpr uint32_t ROW = TC_N * sizeof(Code), PIECES = ROW / 16;
+    static constexpr uint32_t B_PITCH = TC_N * 2 + 16, PAIR_PITCH = TC_N + 16;   // bytes; words
+    uint32_t x_pitch, x, B, pairs, total;   // bytes from the start; codes are first
+    __host__ __device__ TcShared(uint32_t rows) {   // rows: heads * P
+        x_pitch = rows * 2 + 16;
+        x = rows * ROW;
+        B = x + KB * 16 * x_pitch;
+        pairs = B + KB * 16 * B_PITCH;
+        total = pairs + KB * 8 * PAIR_PITCH * 4;
+    }
+    static __device__ __forceinline__ uint32_t swap(uint32_t row) { return (row & 1) << 2 | (row >> 1 & 3); }
+    static __device__ __forceinline__ uint32_t piece(uint32_t row, uint32_t i) { return row * ROW + ((i ^ swap(row)) << 4); }
+    // codes n .. n + 3 of a row
+    static __device__ __forceinline__ uint32_t word(uint32_t row, uint32_t n) {
+        const uint32_t at = n * sizeof(Code);
+        return piece(row, at >> 4) + (at & 15);
+    }
+};
+
+__device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
 // KB: blocks of 16 window tokens (W <= 16 * KB).
 template <typename Code, int MODE, int KB>
-__global__ void __launch_bounds__(TC_THREADS) k_state_tc(StateCacheArgs a) {
+__global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateCacheArgs a, uint32_t heads) {
     constexpr float Q = sizeof(Code) == 1 ? 127.0f : 32767.0f;
-    constexpr int PITCH = MODE == 1 ? TC_N + 16 : TC_N + 4;   // spreads the lanes' rows over the banks
-    __shared__ float s_w[32], s_cb[32], s_alpha;
-    __shared__ uint32_t s_B[KB * 8][PITCH];   // tokens 2 jp and 2 jp + 1 of the window, side by side
-    const uint32_t h = blockIdx.x % a.H, b = blockIdx.x / a.H, g0 = h / (a.H / a.G);
+    using Sh = TcShared<Code, KB>;
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ float s_w[TC_HEADS][32], s_alpha[TC_HEADS];
+    __shared__ __align__(16) __half s_C[TC_N];
+    const uint32_t per_group = a.H / a.G, blocks = (per_group + heads - 1) / heads;
+    const uint32_t g0 = blockIdx.x / blocks % a.G, b = blockIdx.x / blocks / a.G, first = blockIdx.x % blocks * heads;
+    const uint32_t h0 = g0 * per_group + first, nh = min(heads, per_group - first);   // heads h0 .. h0 + nh - 1
     const uint32_t tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
-    const uint64_t bh = (uint64_t)b * a.H + h;
-    const uint64_t xrow = (uint64_t)a.H * a.P, brow = (uint64_t)a.G * TC_N;
-    Code* codes = static_cast<Code*>(a.codes) + bh * a.P * TC_N;
-    const uint32_t tiles = a.P / 16;
-    const uint32_t filled = a.fill[bh];
-    RowCodes<Code> u, v;
-    float sc[2];
-    uint32_t tile = wid;
-    auto fetch = [&] {
-        u.template load<MODE>(codes + (uint64_t)(tile * 16 + g) * TC_N, t);
-        v.template load<MODE>(codes + (uint64_t)(tile * 16 + g + 8) * TC_N, t);
-        sc[0] = a.scales[bh * a.P + tile * 16 + g];
-        sc[1] = a.scales[bh * a.P + tile * 16 + g + 8];
-    };
-    if (tile < tiles) fetch();
-    const __half* wx = a.win_x + (uint64_t)b * a.W * xrow + (uint64_t)h * a.P;
-    __half* wB = a.win_B + (uint64_t)b * a.W * brow + (uint64_t)g0 * TC_N;
-    const __half* xn = MODE == 0 ? a.x + b * a.x_bs + (uint64_t)h * a.P : nullptr;
-    const __half* Bn = MODE == 0 ? a.B + b * a.bc_bs + (uint64_t)g0 * TC_N : nullptr;
-    const __half* Cn = MODE == 0 ? a.C + b * a.bc_bs + (uint64_t)g0 * TC_N : nullptr;
-    // the step's token is number n of the window; `count` tokens with it
-    const uint32_t n = MODE == 0 ? min(filled, a.W - 1) : a.W, count = MODE == 0 ? n + 1 : min(filled, a.W);
+    const uint64_t bh0 = (uint64_t)b * a.H + h0, xrow = (uint64_t)a.H * a.P, brow = (uint64_t)a.G * TC_N;
+    const uint32_t rows = nh * a.P;
+    const Sh sh(heads * a.P);
+    const uint32_t sm0 = smem_u32(sm);
+    Code* codes = static_cast<Code*>(a.codes) + bh0 * a.P * TC_N;
+    float* scales = a.scales + bh0 * a.P;
+    for (uint32_t i = tid; i < rows * Sh::PIECES; i += TC_THREADS)
+        copy_async16(sm0 + Sh::piece(i / Sh::PIECES, i % Sh::PIECES), reinterpret_cast<const uint8_t*>(codes) + (uint64_t)i * 16);
+    // A step's token is number n of the window; `count` tokens with it. All heads of a sequence have the same.
+    const uint32_t filled = a.fill[bh0], n = MODE == 0 ? min(filled, a.W - 1) : a.W;
+    const uint32_t count = MODE == 0 ? n + 1 : min(filled, a.W);
     const bool fold = MODE == 0 && count == a.W;
-    if (wid == 3) {
+    const __half* wx = a.win_x + (uint64_t)b * a.W * xrow + (uint64_t)h0 * a.P;
+    __half* wB = a.win_B + (uint64_t)b * a.W * brow + (uint64_t)g0 * TC_N;
+    const __half* xn = MODE == 0 ? a.x + b * a.x_bs + (uint64_t)h0 * a.P : nullptr;
+    const __half* Bn = MODE == 0 ? a.B + b * a.bc_bs + (uint64_t)g0 * TC_N : nullptr;
+    // the window's rows; those behind its tokens are zeros, so that their products are
+    const uint32_t xp = rows / 8, used = MODE == 0 || count ? KB * 16 : 0;   // 16-byte pieces of a row of x
+    for (uint32_t i = tid; i < used * xp; i += TC_THREADS) {
+        const uint32_t j = i / xp, e = i % xp, to = sh.x + j * sh.x_pitch + e * 16;
+        if (j < count) copy_async16(sm0 + to, (MODE == 0 && j == n ? xn : wx + j * xrow) + e * 8);
+        else *reinterpret_cast<uint4*>(sm + to) = make_uint4(0, 0, 0, 0);
+    }
+    for (uint32_t i = tid; i < used * (TC_N / 8); i += TC_THREADS) {
+        const uint32_t j = i / (TC_N / 8), e = i % (TC_N / 8), to = sh.B + j * Sh::B_PITCH + e * 16;
+        if (j < count) copy_async16(sm0 + to, (MODE == 0 && j == n ? Bn : wB + j * brow) + e * 8);
+        else *reinterpret_cast<uint4*>(sm + to) = make_uint4(0, 0, 0, 0);
+    }
+    if (MODE == 0 && tid < TC_N / 8) copy_async16(smem_u32(s_C) + tid * 16, a.C + b * a.bc_bs + (uint64_t)g0 * TC_N + tid * 8);
+    if (wid < nh) {
+        const uint32_t h = h0 + wid;
+        float* win_dt = a.win_dt + (bh0 + wid) * a.W;
         float dt = 0.0f;
-        if (lane < count && lane != n) dt = a.win_dt[bh * a.W + lane];
+        if (lane < count && lane != n) dt = win_dt[lane];
         if (MODE == 0 && lane == n)
             dt = token_dt(__half2float(a.dt_raw[b * a.dt_bs + h]) + __half2float(a.dt_bias[h]), a.dt_min, a.dt_max);
         float wj, al;
         window_weights(-expf(__half2float(a.A_log[h])), dt, lane, count, &wj, &al);
-        s_w[lane] = wj;
-        if (lane == 0) s_alpha = al;
-        if (MODE == 0 && lane == n) a.win_dt[bh * a.W + n] = dt;
+        s_w[wid][lane] = wj;
+        if (lane == 0) s_alpha[wid] = al;
+        if (MODE == 0 && lane == n) win_dt[n] = dt;
     }
-    if (MODE == 0 && wid < KB) {
-        // C . B_j for tokens 16 wid + g and + g + 8; a row beyond the window's tokens is not read
-        float cb[4] = {};
-        const uint32_t j0 = 16 * wid + g, j1 = j0 + 8;
-        const __half* r0 = j0 == n ? Bn : wB + j0 * brow;
-        const __half* r1 = j1 == n ? Bn : wB + j1 * brow;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint4 z = make_uint4(0, 0, 0, 0);
-            const uint4 p0 = j0 < count ? *reinterpret_cast<const uint4*>(r0 + 32 * i + 8 * t) : z;
-            const uint4 p1 = j1 < count ? *reinterpret_cast<const uint4*>(r1 + 32 * i + 8 * t) : z;
-            const uint4 c = *reinterpret_cast<const uint4*>(Cn + 32 * i + 8 * t);
-            mma16816(cb, p0.x, p1.x, p0.y, p1.y, c.x, c.y);
-            mma16816(cb, p0.z, p1.z, p0.w, p1.w, c.z, c.w);
-        }
-        if (t == 0) { s_cb[j0] = cb[0]; s_cb[j1] = cb[2]; }
-    }
-    if (MODE == 1 || fold) {
-        // the window's B, two tokens a word: 8 KB rows of TC_N words
-        for (uint32_t i = tid; i < KB * 8 * (TC_N / 2); i += TC_THREADS) {
-            const uint32_t jp = i / (TC_N / 2), e = i % (TC_N / 2) * 2, j0 = 2 * jp, j1 = j0 + 1;
-            uint32_t p0 = 0, p1 = 0;
-            if (j0 < count) p0 = *reinterpret_cast<const uint32_t*>((MODE == 0 && j0 == n ? Bn : wB + j0 * brow) + e);
-            if (j1 < count) p1 = *reinterpret_cast<const uint32_t*>((MODE == 0 && j1 == n ? Bn : wB + j1 * brow) + e);
-            s_B[jp][e] = __byte_perm(p0, p1, 0x5410);
-            s_B[jp][e + 1] = __byte_perm(p0, p1, 0x7632);
-        }
-    }
-    uint32_t c[16];
-    if (MODE == 0) {
-        constexpr int PER = 16 / sizeof(Code);
-#pragma unroll
-        for (int i = 0; i < (int)(8 * sizeof(Code) / 4); ++i)
-#pragma unroll
-            for (int k = 0; k < PER / 8; ++k) {
-                const uint4 w = *reinterpret_cast<const uint4*>(Cn + tc_k0<Code, 0>(i * PER / 4, t) + 8 * k);
-                const int o = i * PER / 2 + 4 * k;
-                c[o] = w.x; c[o + 1] = w.y; c[o + 2] = w.z; c[o + 3] = w.w;
-            }
-    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
-    const float alpha = s_alpha;
-    for (; tile < tiles; tile += TC_THREADS / 32) {
-        if (tile != wid) fetch();
-        const uint32_t p0 = tile * 16 + g;
-        // w_j x_j[p] of this lane's tokens 16 k + {2t, 2t + 1, 2t + 8, 2t + 9}, rows g and g + 8
-        float xw[KB][4][2], ywin[2] = {};
+    uint32_t(*pairs)[Sh::PAIR_PITCH] = reinterpret_cast<uint32_t(*)[Sh::PAIR_PITCH]>(sm + sh.pairs);
+    if (MODE == 1 ? count > 0 : fold) {
+        // tokens 2 jp and 2 jp + 1 of the window's B side by side, as the product wants them
+        for (uint32_t i = tid; i < KB * 8 * (TC_N / 2); i += TC_THREADS) {
+            const uint32_t jp = i / (TC_N / 2), e = i % (TC_N / 2) * 2;
+            const uint8_t* from = sm + sh.B + 2 * jp * Sh::B_PITCH + e * 2;
+            const uint32_t p0 = *reinterpret_cast<const uint32_t*>(from), p1 = *reinterpret_cast<const uint32_t*>(from + Sh::B_PITCH);
+            pairs[jp][e] = __byte_perm(p0, p1, 0x5410);
+            pairs[jp][e + 1] = __byte_perm(p0, p1, 0x7632);
+        }
+        __syncthreads();
+    }
+    // C . B_j: rows j = g and g + 8 of every block, in every warp
+    float cb[KB][2];
+    if constexpr (MODE == 0) {
+#pragma unroll
+        for (int k = 0; k < KB; ++k) {
+            float d[4] = {};
+            const uint8_t* r0 = sm + sh.B + (16 * k + g) * Sh::B_PITCH + 16 * t;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4 p0 = lds16(r0 + 64 * i), p1 = lds16(r0 + 8 * Sh::B_PITCH + 64 * i);
+                const uint4 c = lds16(reinterpret_cast<const uint8_t*>(s_C) + 64 * i + 16 * t);
+                mma16816(d, p0.x, p1.x, p0.y, p1.y, c.x, c.y);
+                mma16816(d, p0.z, p1.z, p0.w, p1.w, c.z, c.w);
+            }
+            cb[k][0] = d[0];
+            cb[k][1] = d[2];
+        }
+    }
+    for (uint32_t tile = wid; tile < rows / 16; tile += TC_WARPS) {
+        const uint32_t row = tile * 16 + g, hh = tile * 16 / a.P;   // rows of the CTA's heads
+        const float alpha = s_alpha[hh], sc[2] = {scales[row], scales[row + 8]};
+        // x of the window: a0 (row g; tokens 2t, 2t + 1), a1 (g + 8; same), a2 (g; 2t + 8, + 9), a3 (g + 8; same)
+        uint32_t X[KB][4];
+#pragma unroll
+        for (int k = 0; k < KB; ++k)
+            if (MODE == 0 || count)
+                ldmatrix_t(X[k], sm0 + sh.x + (16 * k + (lane & 7) + (lane >> 4 & 1) * 8) * sh.x_pitch + (tile * 16 + (lane >> 3 & 1) * 8) * 2);
+        if constexpr (MODE == 0) {
+            // the window's part of y: x times w_j (C . B_j), the factor in two f16 terms
+            float wcb[2 * KB];
+#pragma unroll
+            for (int k = 0; k < KB; ++k) {
+                wcb[2 * k] = s_w[hh][16 * k + g] * cb[k][0];
+                wcb[2 * k + 1] = s_w[hh][16 * k + g + 8] * cb[k][1];
+            }
+            const Pow2 p2(wcb);
+            float dw[4] = {};
+#pragma unroll
+            for (int k = 0; k < KB; ++k) {
+                uint32_t hi[2], lo[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {   // tokens 2t, 2t + 1 (+ 8) from the lanes of their rows
+                    const float f0 = __shfl_sync(0xffffffffu, wcb[2 * k + i], 8 * t), f1 = __shfl_sync(0xffffffffu, wcb[2 * k + i], 8 * t + 4);
+                    split2(f0 * p2.up, f1 * p2.up, &hi[i], &lo[i]);
+                }
+                mma16816(dw, X[k][0], X[k][1], X[k][2], X[k][3], hi[0], hi[1]);
+                mma16816(dw, X[k][0], X[k][1], X[k][2], X[k][3], lo[0], lo[1]);
+            }
+            // S_q C: lane t's word q is codes k0 .. k0 + 3 of both rows
+            float lo[4] = {}, hi[4] = {};
+#pragma unroll
+            for (int i = 0; i < (int)(8 * sizeof(Code) / 4); ++i) {
+                // 16 bytes a row: pieces 4 i + t
+                const uint4 u4 = lds16(sm + Sh::piece(row, 4 * i + t)), v4 = lds16(sm + Sh::piece(row + 8, 4 * i + t));
+                const uint32_t u[4] = {u4.x, u4.y, u4.z, u4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
+                constexpr int PER = 16 / sizeof(Code);   // codes a piece
+                uint32_t c[PER / 2];
+#pragma unroll
+                for (int k = 0; k < PER / 8; ++k) {
+                    const uint4 w = lds16(reinterpret_cast<const uint8_t*>(s_C) + ((4 * i + t) * PER + 8 * k) * 2);
+                    c[4 * k] = w.x; c[4 * k + 1] = w.y; c[4 * k + 2] = w.z; c[4 * k + 3] = w.w;
+                }
+                if constexpr (sizeof(Code) == 1) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const uint32_t x = u[q] ^ 0x80808080u, y = v[q] ^ 0x80808080u;
+                        mma16816(lo, bytes_h2(x, 0x4140, 1152.0f), bytes_h2(y, 0x4140, 1152.0f), bytes_h2(x, 0x4342, 1152.0f),
+                                 bytes_h2(y, 0x4342, 1152.0f), c[2 * q], c[2 * q + 1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const uint32_t x0 = u[2 * q], x1 = u[2 * q + 1], y0 = v[2 * q], y1 = v[2 * q + 1];
+                        mma16816(lo, bytes_h2(x0, 0x4240, 1024.0f), bytes_h2(y0, 0x4240, 1024.0f), bytes_h2(x1, 0x4240, 1024.0f),
+                                 bytes_h2(y1, 0x4240, 1024.0f), c[2 * q], c[2 * q + 1]);
+                        mma16816(hi, bytes_h2(x0 ^ 0x80008000u, 0x4341, 1152.0f), bytes_h2(y0 ^ 0x80008000u, 0x4341, 1152.0f),
+                                 bytes_h2(x1 ^ 0x80008000u, 0x4341, 1152.0f), bytes_h2(y1 ^ 0x80008000u, 0x4341, 1152.0f), c[2 * q],
+                                 c[2 * q + 1]);
+                    }
+                }
+            }
+            if (t < 2) {   // lane t = 0 has row g, t = 1 row g + 8
+                const float low = t ? lo[2] : lo[0], dot = sizeof(Code) == 1 ? low : fmaf(256.0f, t ? hi[2] : hi[0], low);
+                const uint32_t h = h0 + hh, p = row + 8 * t;
+                const uint64_t o = (uint64_t)h0 * a.P + p;
+                const __half xh = *reinterpret_cast<const __half*>(sm + sh.x + n * sh.x_pitch + p * 2);
+                const float Dh = a.has_D ? __half2float(a.D[h]) : 0.0f;
+                const __half yh = __float2half_rn(fmaf(alpha * (t ? sc[1] : sc[0]), dot, (t ? dw[2] : dw[0]) * p2.down) + Dh * __half2float(xh));
+                a.y[b * a.y_bs + o] = a.z ? __float2half_rn(silu(__half2float(a.z[b * a.z_bs + o])) * __half2float(yh)) : yh;
+                a.win_x[((uint64_t)b * a.W + n) * xrow + o] = xh;
+            }
+            if (!fold) continue;
+        }
+        // the window's part of the state: w_j x_j[p] in two f16 terms, scaled, times the window's B
+        float xw[KB * 8];
 #pragma unroll
         for (int k = 0; k < KB; ++k)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t j = 16 * k + 2 * t + (i & 1) + 8 * (i >> 1);
-                const __half* xj = MODE == 0 && j == n ? xn : wx + j * xrow;
-                const float wj = s_w[j];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float x = j < count ? __half2float(xj[p0 + 8 * r]) : 0.0f;
-                    xw[k][i][r] = wj * x;
-                    if (MODE == 0 && j < count) ywin[r] = fmaf(s_cb[j], xw[k][i][r], ywin[r]);
-                }
+                const float2 f = MODE == 0 || count ? __half22float2(bits_h2(X[k][i])) : make_float2(0.0f, 0.0f);
+                const uint32_t j = 16 * k + 2 * t + 8 * (i >> 1);
+                xw[8 * k + 2 * i] = s_w[hh][j] * f.x;
+                xw[8 * k + 2 * i + 1] = s_w[hh][j + 1] * f.y;
             }
-        if (MODE == 0) {
-            float y[2];
-            codes_dot_c(u, v, c, y);
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                ywin[r] += __shfl_xor_sync(0xffffffffu, ywin[r], 1);
-                ywin[r] += __shfl_xor_sync(0xffffffffu, ywin[r], 2);
-                if (t == r) {
-                    const uint64_t o = (uint64_t)h * a.P + p0 + 8 * r;
-                    const __half xh = xn[p0 + 8 * r];
-                    const float Dh = a.has_D ? __half2float(a.D[h]) : 0.0f;
-                    const __half yh = __float2half_rn(fmaf(alpha * sc[r], y[r], ywin[r]) + Dh * __half2float(xh));
-                    a.y[b * a.y_bs + o] =
-                        a.z ? __float2half_rn(silu(__half2float(a.z[b * a.z_bs + o])) * __half2float(yh)) : yh;
-                    a.win_x[((uint64_t)b * a.W + n) * xrow + o] = xh;
-                }
-            }
-            if (!fold) continue;
-        }
-        // the window's part of the state. Terms that are not finite set no scale, and come out as they are.
-        uint32_t top = 0;
-#pragma unroll
-        for (int k = 0; k < KB; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t bits = __float_as_uint(xw[k][i / 2][i % 2]) & 0x7FFFFFFFu;
-                if (bits < 0x7F800000u) top = max(top, bits);
-            }
-        const uint32_t eb = max(__reduce_max_sync(0xffffffffu, top) >> 23, 15u);
-        const float up = __uint_as_float(min(268u - eb, 254u) << 23), down = __uint_as_float((eb - 14u) << 23);
+        const Pow2 p2(xw);
         uint32_t ah[KB][4], al[KB][4];
 #pragma unroll
         for (int k = 0; k < KB; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // a0 (g; 2t, 2t + 1), a1 (g + 8; same), a2 (g; 2t + 8, + 9), a3 (g + 8; same)
-                const int r = i & 1, at = i & 2;
-                const float x0 = xw[k][at][r] * up, x1 = xw[k][at + 1][r] * up;
-                const __half2 hh = __floats2half2_rn(x0, x1);
-                const float2 f = __half22float2(hh);
-                ah[k][i] = h2_bits(hh);
-                al[k][i] = h2_bits(__floats2half2_rn(x0 - f.x, x1 - f.y));
-            }
-        const float as0 = alpha * sc[0], as1 = alpha * sc[1];
-        // word q of the state, rows g and g + 8
+            for (int i = 0; i < 4; ++i) split2(xw[8 * k + 2 * i] * p2.up, xw[8 * k + 2 * i + 1] * p2.up, &ah[k][i], &al[k][i]);
+        const float as[2] = {alpha * sc[0], alpha * sc[1]};
+        // elements 16 q + 4 t .. + 3 of the state, rows g and g + 8
         auto word = [&](int q, float (&s)[2][4]) {
             float cu[4], cv[4];
-            u.values(q, cu);
-            v.values(q, cv);
+            code_values<Code>(sm + Sh::word(row, 16 * q + 4 * t), cu);
+            code_values<Code>(sm + Sh::word(row + 8, 16 * q + 4 * t), cv);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
+                // column c of the product is element 16 q + 4 (c / 2) + c % 2 + 2 half: a lane gets what its codes are
                 float d[4] = {};
-                const int e = tc_k0<Code, MODE>(q, g >> 1) + (g & 1) + 2 * half;
+                const int e = 16 * q + 4 * (g >> 1) + (g & 1) + 2 * half;
+                if (MODE == 0 || count) {
 #pragma unroll
-                for (int k = 0; k < KB; ++k) {
-                    const uint32_t b0 = s_B[8 * k + t][e], b1 = s_B[8 * k + t + 4][e];
-                    mma16816(d, ah[k][0], ah[k][1], ah[k][2], ah[k][3], b0, b1);
-                    mma16816(d, al[k][0], al[k][1], al[k][2], al[k][3], b0, b1);
+                    for (int k = 0; k < KB; ++k) {
+                        const uint32_t b0 = pairs[8 * k + t][e], b1 = pairs[8 * k + t + 4][e];
+                        mma16816(d, ah[k][0], ah[k][1], ah[k][2], ah[k][3], b0, b1);
+                        mma16816(d, al[k][0], al[k][1], al[k][2], al[k][3], b0, b1);
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    s[0][2 * half + i] = fmaf(d[i], down, as0 * cu[2 * half + i]);
-                    s[1][2 * half + i] = fmaf(d[2 + i], down, as1 * cv[2 * half + i]);
+                    s[0][2 * half + i] = fmaf(d[i], p2.down, as[0] * cu[2 * half + i]);
+                    s[1][2 * half + i] = fmaf(d[2 + i], p2.down, as[1] * cv[2 * half + i]);
                 }
             }
         };
         if constexpr (MODE == 1) {
-#pragma unroll
+#pragma unroll 2
             for (int q = 0; q < 8; ++q) {
                 float s[2][4];
                 word(q, s);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const uint64_t o = (bh * a.P + p0 + 8 * r) * TC_N + tc_k0<Code, 1>(q, t);
+                    const uint64_t o = (bh0 * a.P + row + 8 * r) * TC_N + 16 * q + 4 * t;
                     if (a.state_dtype == LSSM_DT_F32)
                         __stcs(reinterpret_cast<float4*>(static_cast<float*>(a.state) + o), make_float4(s[r][0], s[r][1], s[r][2], s[r][3]));
                     else {
@@ -466,66 +539,79 @@ __global__ void __launch_bounds__(TC_THREADS) k_state_tc(StateCacheArgs a) {
                 }
             }
         } else {
-            // the rows' largest elements first, then the codes: computed twice, once in W steps, instead of
-            // held in 64 registers at every step
-            float amax0 = 0.0f, amax1 = 0.0f;
-#pragma unroll
+            // The rows' largest elements first, then the codes: computed twice, once in W steps, so that no step
+            // holds the registers for it.
+            float amax[2] = {};
+#pragma unroll 1
             for (int q = 0; q < 8; ++q) {
                 float s[2][4];
                 word(q, s);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    amax0 = max_keep_nan(amax0, fabsf(s[0][i]));
-                    amax1 = max_keep_nan(amax1, fabsf(s[1][i]));
-                }
+                for (int i = 0; i < 8; ++i) amax[i / 4] = max_keep_nan(amax[i / 4], fabsf(s[i / 4][i % 4]));
             }
 #pragma unroll
-            for (int o = 1; o <= 2; o <<= 1) {
-                amax0 = max_keep_nan(amax0, __shfl_xor_sync(0xffffffffu, amax0, o));
-                amax1 = max_keep_nan(amax1, __shfl_xor_sync(0xffffffffu, amax1, o));
-            }
-            const float n0 = row_scale(amax0, Q), n1 = row_scale(amax1, Q);
-            const float i0 = n0 > 0.0f ? 1.0f / n0 : 0.0f, i1 = n1 > 0.0f ? 1.0f / n1 : 0.0f;
+            for (int o = 1; o <= 2; o <<= 1)
 #pragma unroll
+                for (int r = 0; r < 2; ++r) amax[r] = max_keep_nan(amax[r], __shfl_xor_sync(0xffffffffu, amax[r], o));
+            const RowQuant z0(amax[0], Q), z1(amax[1], Q);
+#pragma unroll 1
             for (int q = 0; q < 8; ++q) {
                 float s[2][4];
-                int c0[4], c1[4];
                 word(q, s);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    c0[i] = nearest_code(s[0][i], n0, i0, Q);
-                    c1[i] = nearest_code(s[1][i], n1, i1, Q);
-                }
-                u.set(q, c0);
-                v.set(q, c1);
+                store_codes4(reinterpret_cast<Code*>(sm + Sh::word(row, 16 * q + 4 * t)), s[0], z0);
+                store_codes4(reinterpret_cast<Code*>(sm + Sh::word(row + 8, 16 * q + 4 * t)), s[1], z1);
             }
-            u.store(codes + (uint64_t)p0 * TC_N, t);
-            v.store(codes + (uint64_t)(p0 + 8) * TC_N, t);
             if (t == 0) {
-                a.scales[bh * a.P + p0] = n0;
-                a.scales[bh * a.P + p0 + 8] = n1;
+                scales[row] = z0.scale;
+                scales[row + 8] = z1.scale;
+            }
+            __syncwarp();
+            for (uint32_t i = lane; i < 16 * Sh::PIECES; i += 32) {
+                const uint32_t rr = tile * 16 + i / Sh::PIECES, q = i % Sh::PIECES;
+                *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(codes) + (uint64_t)rr * Sh::ROW + q * 16) = lds16(sm + Sh::piece(rr, q));
             }
         }
     }
     if (MODE == 0) {
         // the first head of a group keeps the group's B row; every head takes row n from its argument
-        if (h % (a.H / a.G) == 0 && tid < TC_N / 8)
-            *reinterpret_cast<uint4*>(wB + n * brow + 8 * tid) = *reinterpret_cast<const uint4*>(Bn + 8 * tid);
-        if (tid == 0) a.fill[bh] = fold ? 0 : n + 1;
+        if (first == 0 && tid < TC_N / 8)
+            *reinterpret_cast<uint4*>(wB + n * brow + 8 * tid) = lds16(sm + sh.B + n * Sh::B_PITCH + 16 * tid);
+        if (tid < nh) a.fill[bh0 + tid] = fold ? 0 : count;
     }
+}
+
+template <typename Code, int MODE, int KB>
+cudaError_t launch_tc(const StateCacheArgs& a, uint32_t heads, cudaStream_t s) {
+    const uint32_t bytes = TcShared<Code, KB>(heads * a.P).total;
+    if (bytes > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(k_state_tc<Code, MODE, KB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e != cudaSuccess) return e;
+    }
+    const uint32_t per_group = a.H / a.G;
+    k_state_tc<Code, MODE, KB><<<a.batch * a.G * ((per_group + heads - 1) / heads), TC_THREADS, bytes, s>>>(a, heads);
+    return cudaGetLastError();
 }
 
 template <typename Code, int MODE>
 cudaError_t launch_cached(const StateCacheArgs& a, cudaStream_t s) {
-    const unsigned grid = a.batch * a.H;
-    // 16-byte loads of codes, B and C, 8- or 16-byte stores of the state: rows of 128 keep the base's alignment
-    bool tc = a.N == TC_N && a.P % 16 == 0 && aligned(a.codes, 16) && aligned(a.win_B, 16);
-    if (MODE == 0) tc = tc && aligned(a.B, 16) && aligned(a.C, 16) && a.bc_bs % 8 == 0;
+    // rows of 128 and heads of 16 rows keep the arrays' 16-byte alignment
+    bool tc = a.N == TC_N && a.P % 16 == 0 && a.P <= TC_ROWS && aligned(a.codes, 16) && aligned(a.win_x, 16) && aligned(a.win_B, 16);
+    if (MODE == 0) tc = tc && aligned(a.x, 16) && aligned(a.B, 16) && aligned(a.C, 16) && a.bc_bs % 8 == 0 && a.x_bs % 8 == 0;
     else tc = tc && aligned(a.state, 16);
-    if (tc && a.W <= 16) k_state_tc<Code, MODE, 1><<<grid, TC_THREADS, 0, s>>>(a);
-    else if (tc) k_state_tc<Code, MODE, 2><<<grid, TC_THREADS, 0, s>>>(a);
-    else k_state_cached<Code, MODE><<<grid, SC_THREADS, 0, s>>>(a);
-    return cudaGetLastError();
+    if (!tc) {
+        k_state_cached<Code, MODE><<<a.batch * a.H, SC_THREADS, 0, s>>>(a);
+        return cudaGetLastError();
+    }
+    // Heads of a group share the window's B and what is computed from it: as many as 32 KB of codes allow, fewer
+    // where the grid would leave SMs without a CTA.
+    const uint32_t per_group = a.H / a.G;
+    uint32_t heads = TC_HEADS;
+    while (heads > 1 && (heads * a.P > TC_ROWS / sizeof(Code) ||
+                         (uint64_t)a.batch * a.G * ((per_group + heads - 1) / heads) < 2ull * 148)) heads /= 2;
+#ifdef SCENV
+    if (getenv("SC_HEADS")) heads = atoi(getenv("SC_HEADS"));
+#endif
+    return a.W <= 16 ? launch_tc<Code, MODE, 1>(a, heads, s) : launch_tc<Code, MODE, 2>(a, heads, s);
 }
 
 template <typename Code>
@@ -538,10 +624,10 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_store(StateCacheArgs a) {
     Code* out = static_cast<Code*>(a.codes) + row * a.N;
     float amax = 0.0f;
     for (uint32_t i = lane; i < a.N; i += 32) amax = max_nan(amax, fabsf(S[i]));
-    const float scale = row_scale(warp_max_nan(amax), Q), inv = scale > 0.0f ? 1.0f / scale : 0.0f;
-    for (uint32_t i = lane; i < a.N; i += 32) out[i] = (Code)nearest_code(S[i], scale, inv, Q);
+    const RowQuant z(warp_max_nan(amax), Q);
+    for (uint32_t i = lane; i < a.N; i += 32) out[i] = quantise1<Code>(S[i], z);
     if (lane == 0) {
-        a.scales[row] = scale;
+        a.scales[row] = z.scale;
         if (row % a.P == 0) a.fill[row / a.P] = 0;
     }
 }
@@ -567,17 +653,10 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_store128(StateCacheArgs a)
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(e[i]) & 0x7FFFFFFFu);
-        const float scale = row_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, top)), Q);
-        const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
-        int c[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = nearest_code(e[i], scale, inv, Q);
-        if constexpr (sizeof(Code) == 1)
-            *reinterpret_cast<uint32_t*>(out + r * 128) = (c[0] & 0xFF) | (c[1] & 0xFF) << 8 | (c[2] & 0xFF) << 16 | (uint32_t)c[3] << 24;
-        else
-            *reinterpret_cast<uint2*>(out + r * 128) = make_uint2((c[0] & 0xFFFF) | (uint32_t)c[1] << 16, (c[2] & 0xFFFF) | (uint32_t)c[3] << 16);
+        const RowQuant z(__uint_as_float(__reduce_max_sync(0xffffffffu, top)), Q);
+        store_codes4(out + r * 128, e, z);
         if (lane == 0) {
-            a.scales[row0 + r] = scale;
+            a.scales[row0 + r] = z.scale;
             if ((row0 + r) % a.P == 0) a.fill[(row0 + r) / a.P] = 0;
         }
     }
