@@ -216,6 +216,10 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_cached(StateCacheArgs a) {
 // codes' bytes and the latency of a short CTA.
 constexpr int TC_THREADS = 256, TC_WARPS = TC_THREADS / 32, TC_N = 128, TC_HEADS = 4;
 constexpr uint32_t TC_ROWS = 256;   // rows of 8-bit codes a CTA holds (32 KB)
+#ifndef SCC
+#define SCC 4
+#endif
+constexpr int TC_CTAS = SCC;
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -287,100 +291,115 @@ struct Pow2 {
 };
 
 // Shared memory of a CTA: the heads' codes (rows of TC_N, their 16-byte pieces exchanged by row so that neither
-// 16-byte nor 4-byte reads of 8 rows meet in a bank), the window's x (a row a token) and B, the pair layout of B.
+// 16-byte nor 4-byte reads of 8 rows meet in a bank), the window's x (a row a token) and B, C, and the pair layout of B.
 template <typename Code, int KB>
 struct TcShared {
     static constexpr uint32_t ROW = TC_N * sizeof(Code), PIECES = ROW / 16;
     static constexpr uint32_t B_PITCH = TC_N * 2 + 16, PAIR_PITCH = TC_N + 16;   // bytes; words
-    uint32_t x_pitch, x, B, pairs, total;   // bytes from the start; codes are first
+    uint32_t x_pitch, x, B, C, pairs, total;   // bytes from the start; codes are first
     __host__ __device__ TcShared(uint32_t rows) {   // rows: heads * P
         x_pitch = rows * 2 + 16;
         x = rows * ROW;
         B = x + KB * 16 * x_pitch;
-        pairs = B + KB * 16 * B_PITCH;
+        C = B + KB * 16 * B_PITCH;
+        pairs = C + TC_N * 2;
         total = pairs + KB * 8 * PAIR_PITCH * 4;
     }
     static __device__ __forceinline__ uint32_t swap(uint32_t row) { return (row & 1) << 2 | (row >> 1 & 3); }
     static __device__ __forceinline__ uint32_t piece(uint32_t row, uint32_t i) { return row * ROW + ((i ^ swap(row)) << 4); }
-    // codes n .. n + 3 of a row
-    static __device__ __forceinline__ uint32_t word(uint32_t row, uint32_t n) {
-        const uint32_t at = n * sizeof(Code);
-        return piece(row, at >> 4) + (at & 15);
-    }
 };
 
 __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
-// KB: blocks of 16 window tokens (W <= 16 * KB).
+// KB: blocks of 16 window tokens (W <= 16 * KB). Grid: blocks of heads, groups, sequences.
 template <typename Code, int MODE, int KB>
-__global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateCacheArgs a, uint32_t heads) {
+__global__ void __launch_bounds__(TC_THREADS, TC_CTAS) k_state_tc(StateCacheArgs a, uint32_t heads) {
     constexpr float Q = sizeof(Code) == 1 ? 127.0f : 32767.0f;
     using Sh = TcShared<Code, KB>;
     extern __shared__ __align__(128) uint8_t sm[];
-    __shared__ float s_w[TC_HEADS][32], s_alpha[TC_HEADS];
-    __shared__ __align__(16) __half s_C[TC_N];
-    const uint32_t per_group = a.H / a.G, blocks = (per_group + heads - 1) / heads;
-    const uint32_t g0 = blockIdx.x / blocks % a.G, b = blockIdx.x / blocks / a.G, first = blockIdx.x % blocks * heads;
-    const uint32_t h0 = g0 * per_group + first, nh = min(heads, per_group - first);   // heads h0 .. h0 + nh - 1
+    __shared__ __align__(8) float s_w[TC_HEADS][32];
+    __shared__ float s_alpha[TC_HEADS], s_D[TC_HEADS];
+    const uint32_t per_group = a.H / a.G, first = blockIdx.x * heads, nh = min(heads, per_group - first), b = blockIdx.z;
+    const uint32_t h0 = blockIdx.y * per_group + first;   // heads h0 .. h0 + nh - 1
     const uint32_t tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
-    const uint64_t bh0 = (uint64_t)b * a.H + h0, xrow = (uint64_t)a.H * a.P, brow = (uint64_t)a.G * TC_N;
-    const uint32_t rows = nh * a.P;
+    const uint32_t rows = nh * a.P, bh0 = b * a.H + h0;
+    const uint32_t xrow = a.H * a.P, brow = a.G * TC_N;
     const Sh sh(heads * a.P);
     const uint32_t sm0 = smem_u32(sm);
-    Code* codes = static_cast<Code*>(a.codes) + bh0 * a.P * TC_N;
-    float* scales = a.scales + bh0 * a.P;
-    for (uint32_t i = tid; i < rows * Sh::PIECES; i += TC_THREADS)
-        copy_async16(sm0 + Sh::piece(i / Sh::PIECES, i % Sh::PIECES), reinterpret_cast<const uint8_t*>(codes) + (uint64_t)i * 16);
-    // A step's token is number n of the window; `count` tokens with it. All heads of a sequence have the same.
-    const uint32_t filled = a.fill[bh0], n = MODE == 0 ? min(filled, a.W - 1) : a.W;
-    const uint32_t count = MODE == 0 ? n + 1 : min(filled, a.W);
-    const bool fold = MODE == 0 && count == a.W;
-    const __half* wx = a.win_x + (uint64_t)b * a.W * xrow + (uint64_t)h0 * a.P;
-    __half* wB = a.win_B + (uint64_t)b * a.W * brow + (uint64_t)g0 * TC_N;
-    const __half* xn = MODE == 0 ? a.x + b * a.x_bs + (uint64_t)h0 * a.P : nullptr;
-    const __half* Bn = MODE == 0 ? a.B + b * a.bc_bs + (uint64_t)g0 * TC_N : nullptr;
-    // the window's rows; those behind its tokens are zeros, so that their products are
-    const uint32_t xp = rows / 8, used = MODE == 0 || count ? KB * 16 : 0;   // 16-byte pieces of a row of x
-    for (uint32_t i = tid; i < used * xp; i += TC_THREADS) {
-        const uint32_t j = i / xp, e = i % xp, to = sh.x + j * sh.x_pitch + e * 16;
-        if (j < count) copy_async16(sm0 + to, (MODE == 0 && j == n ? xn : wx + j * xrow) + e * 8);
-        else *reinterpret_cast<uint4*>(sm + to) = make_uint4(0, 0, 0, 0);
+    uint8_t* codes = static_cast<uint8_t*>(a.codes) + (uint64_t)bh0 * a.P * Sh::ROW;
+    float* scales = a.scales + (uint64_t)bh0 * a.P;
+    const uint32_t filled = a.fill[bh0];
+    {
+        const uint8_t* from = codes + tid * 16;
+        constexpr uint32_t STEP = TC_THREADS / Sh::PIECES;   // rows a round, a multiple of 8: the exchange repeats
+        uint32_t to = sm0 + Sh::piece(tid / Sh::PIECES, tid % Sh::PIECES);
+        for (uint32_t r = tid / Sh::PIECES; r < rows; r += STEP, from += TC_THREADS * 16, to += TC_THREADS * 16) copy_async16(to, from);
     }
-    for (uint32_t i = tid; i < used * (TC_N / 8); i += TC_THREADS) {
-        const uint32_t j = i / (TC_N / 8), e = i % (TC_N / 8), to = sh.B + j * Sh::B_PITCH + e * 16;
-        if (j < count) copy_async16(sm0 + to, (MODE == 0 && j == n ? Bn : wB + j * brow) + e * 8);
-        else *reinterpret_cast<uint4*>(sm + to) = make_uint4(0, 0, 0, 0);
-    }
-    if (MODE == 0 && tid < TC_N / 8) copy_async16(smem_u32(s_C) + tid * 16, a.C + b * a.bc_bs + (uint64_t)g0 * TC_N + tid * 8);
+    // what warp w < nh needs for head w's weights; scales of this warp's first tile
+    float p_dt = 0.0f, p_raw = 0.0f, p_bias = 0.0f, p_A = 0.0f, p_D = 0.0f, sc[2] = {};
     if (wid < nh) {
         const uint32_t h = h0 + wid;
-        float* win_dt = a.win_dt + (bh0 + wid) * a.W;
-        float dt = 0.0f;
-        if (lane < count && lane != n) dt = win_dt[lane];
-        if (MODE == 0 && lane == n)
-            dt = token_dt(__half2float(a.dt_raw[b * a.dt_bs + h]) + __half2float(a.dt_bias[h]), a.dt_min, a.dt_max);
+        if (lane < a.W) p_dt = a.win_dt[(uint64_t)(bh0 + wid) * a.W + lane];
+        p_A = __half2float(a.A_log[h]);
+        if (MODE == 0) {
+            p_raw = __half2float(a.dt_raw[b * a.dt_bs + h]);
+            p_bias = __half2float(a.dt_bias[h]);
+            if (a.has_D) p_D = __half2float(a.D[h]);
+        }
+    }
+    if (wid < rows / 16) { sc[0] = scales[wid * 16 + g]; sc[1] = scales[wid * 16 + g + 8]; }
+    // A step's token is number n of the window; `count` tokens with it. All heads of a sequence have the same.
+    const uint32_t n = MODE == 0 ? min(filled, a.W - 1) : a.W, count = MODE == 0 ? n + 1 : min(filled, a.W);
+    const bool fold = MODE == 0 && count == a.W;
+    const __half* wx = a.win_x + ((uint64_t)b * a.W * xrow + (uint64_t)h0 * a.P);
+    __half* wB = a.win_B + ((uint64_t)b * a.W * brow + blockIdx.y * TC_N);
+    const __half* xn = MODE == 0 ? a.x + b * a.x_bs + (uint64_t)h0 * a.P : nullptr;
+    const __half* Bn = MODE == 0 ? a.B + b * a.bc_bs + blockIdx.y * TC_N : nullptr;
+    // the window's rows, a warp each of x, half a warp each of B; those behind its tokens are zeros, so that their
+    // products are
+    if (MODE == 0 || count) {
+        for (uint32_t j = wid; j < KB * 16; j += TC_WARPS) {
+            const __half* from = MODE == 0 && j == n ? xn : wx + (uint64_t)j * xrow;
+            const uint32_t to = sh.x + j * sh.x_pitch;
+            for (uint32_t e = lane; e < rows / 8; e += 32) {
+                if (j < count) copy_async16(sm0 + to + e * 16, from + e * 8);
+                else *reinterpret_cast<uint4*>(sm + to + e * 16) = make_uint4(0, 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < KB; ++k) {
+            const uint32_t j = 16 * k + tid / 16, e = tid % 16, to = sh.B + j * Sh::B_PITCH + e * 16;
+            if (j < count) copy_async16(sm0 + to, (MODE == 0 && j == n ? Bn : wB + (uint64_t)j * brow) + e * 8);
+            else *reinterpret_cast<uint4*>(sm + to) = make_uint4(0, 0, 0, 0);
+        }
+    }
+    if (MODE == 0 && tid < TC_N / 8) copy_async16(sm0 + sh.C + tid * 16, a.C + b * a.bc_bs + blockIdx.y * TC_N + tid * 8);
+    if (wid < nh) {
+        float dt = lane < count ? p_dt : 0.0f;
+        if (MODE == 0 && lane == n) dt = token_dt(p_raw + p_bias, a.dt_min, a.dt_max);
         float wj, al;
-        window_weights(-expf(__half2float(a.A_log[h])), dt, lane, count, &wj, &al);
+        window_weights(-expf(p_A), dt, lane, count, &wj, &al);
         s_w[wid][lane] = wj;
-        if (lane == 0) s_alpha[wid] = al;
-        if (MODE == 0 && lane == n) win_dt[n] = dt;
+        if (lane == 0) { s_alpha[wid] = al; s_D[wid] = p_D; }
+        if (MODE == 0 && lane == n) a.win_dt[(uint64_t)(bh0 + wid) * a.W + n] = dt;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     uint32_t(*pairs)[Sh::PAIR_PITCH] = reinterpret_cast<uint32_t(*)[Sh::PAIR_PITCH]>(sm + sh.pairs);
     if (MODE == 1 ? count > 0 : fold) {
         // tokens 2 jp and 2 jp + 1 of the window's B side by side, as the product wants them
+#pragma unroll
         for (uint32_t i = tid; i < KB * 8 * (TC_N / 2); i += TC_THREADS) {
             const uint32_t jp = i / (TC_N / 2), e = i % (TC_N / 2) * 2;
             const uint8_t* from = sm + sh.B + 2 * jp * Sh::B_PITCH + e * 2;
             const uint32_t p0 = *reinterpret_cast<const uint32_t*>(from), p1 = *reinterpret_cast<const uint32_t*>(from + Sh::B_PITCH);
-            pairs[jp][e] = __byte_perm(p0, p1, 0x5410);
-            pairs[jp][e + 1] = __byte_perm(p0, p1, 0x7632);
+            *reinterpret_cast<uint2*>(&pairs[jp][e]) = make_uint2(__byte_perm(p0, p1, 0x5410), __byte_perm(p0, p1, 0x7632));
         }
         __syncthreads();
     }
-    // C . B_j: rows j = g and g + 8 of every block, in every warp
-    float cb[KB][2];
+    // C . B_j in every warp: rows j = g and g + 8 of every block, then to the lanes that use them: tokens
+    // 16 k + {2t, 2t + 1, 2t + 8, 2t + 9}
+    float cb[KB][4];
     if constexpr (MODE == 0) {
 #pragma unroll
         for (int k = 0; k < KB; ++k) {
@@ -388,57 +407,58 @@ __global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateC
             const uint8_t* r0 = sm + sh.B + (16 * k + g) * Sh::B_PITCH + 16 * t;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint4 p0 = lds16(r0 + 64 * i), p1 = lds16(r0 + 8 * Sh::B_PITCH + 64 * i);
-                const uint4 c = lds16(reinterpret_cast<const uint8_t*>(s_C) + 64 * i + 16 * t);
+                const uint4 p0 = lds16(r0 + 64 * i), p1 = lds16(r0 + 8 * Sh::B_PITCH + 64 * i), c = lds16(sm + sh.C + 64 * i + 16 * t);
                 mma16816(d, p0.x, p1.x, p0.y, p1.y, c.x, c.y);
                 mma16816(d, p0.z, p1.z, p0.w, p1.w, c.z, c.w);
             }
-            cb[k][0] = d[0];
-            cb[k][1] = d[2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cb[k][i] = __shfl_sync(0xffffffffu, d[i & 2], 8 * t + 4 * (i & 1));
         }
     }
+    const uint32_t ldm = sm0 + sh.x + ((lane & 7) + (lane >> 4 & 1) * 8) * sh.x_pitch + (lane >> 3 & 1) * 16;
     for (uint32_t tile = wid; tile < rows / 16; tile += TC_WARPS) {
         const uint32_t row = tile * 16 + g, hh = tile * 16 / a.P;   // rows of the CTA's heads
-        const float alpha = s_alpha[hh], sc[2] = {scales[row], scales[row + 8]};
-        // x of the window: a0 (row g; tokens 2t, 2t + 1), a1 (g + 8; same), a2 (g; 2t + 8, + 9), a3 (g + 8; same)
-        uint32_t X[KB][4];
+        const float alpha = s_alpha[hh];
+        if (tile != wid) { sc[0] = scales[row]; sc[1] = scales[row + 8]; }
+        const float as[2] = {alpha * sc[0], alpha * sc[1]};
+        // w_j x_j[p] of the lane's tokens: [0], [1] row g, tokens 2t, 2t + 1; [2], [3] row g + 8; [4] .. [7] tokens + 8
+        float xw[KB * 8];
 #pragma unroll
-        for (int k = 0; k < KB; ++k)
-            if (MODE == 0 || count)
-                ldmatrix_t(X[k], sm0 + sh.x + (16 * k + (lane & 7) + (lane >> 4 & 1) * 8) * sh.x_pitch + (tile * 16 + (lane >> 3 & 1) * 8) * 2);
+        for (int k = 0; k < KB; ++k) {
+            uint32_t X[4] = {};
+            if (MODE == 0 || count) ldmatrix_t(X, ldm + 16 * k * sh.x_pitch + tile * 32);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = __half22float2(bits_h2(X[i])), w = *reinterpret_cast<const float2*>(&s_w[hh][16 * k + 2 * t + 8 * (i >> 1)]);
+                xw[8 * k + 2 * i] = w.x * f.x;
+                xw[8 * k + 2 * i + 1] = w.y * f.y;
+            }
+        }
+        const uint32_t sw = Sh::swap(row);   // of row + 8, too
+        const uint8_t* r0 = sm + row * Sh::ROW;
         if constexpr (MODE == 0) {
-            // the window's part of y: x times w_j (C . B_j), the factor in two f16 terms
-            float wcb[2 * KB];
+            float yw[2] = {};
 #pragma unroll
-            for (int k = 0; k < KB; ++k) {
-                wcb[2 * k] = s_w[hh][16 * k + g] * cb[k][0];
-                wcb[2 * k + 1] = s_w[hh][16 * k + g + 8] * cb[k][1];
+            for (int k = 0; k < KB; ++k)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) yw[i >> 1 & 1] = fmaf(xw[8 * k + i], cb[k][(i & 1) + 2 * (i >> 2)], yw[i >> 1 & 1]);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                yw[r] += __shfl_xor_sync(0xffffffffu, yw[r], 1);
+                yw[r] += __shfl_xor_sync(0xffffffffu, yw[r], 2);
             }
-            const Pow2 p2(wcb);
-            float dw[4] = {};
-#pragma unroll
-            for (int k = 0; k < KB; ++k) {
-                uint32_t hi[2], lo[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {   // tokens 2t, 2t + 1 (+ 8) from the lanes of their rows
-                    const float f0 = __shfl_sync(0xffffffffu, wcb[2 * k + i], 8 * t), f1 = __shfl_sync(0xffffffffu, wcb[2 * k + i], 8 * t + 4);
-                    split2(f0 * p2.up, f1 * p2.up, &hi[i], &lo[i]);
-                }
-                mma16816(dw, X[k][0], X[k][1], X[k][2], X[k][3], hi[0], hi[1]);
-                mma16816(dw, X[k][0], X[k][1], X[k][2], X[k][3], lo[0], lo[1]);
-            }
-            // S_q C: lane t's word q is codes k0 .. k0 + 3 of both rows
+            // S_q C: 16 bytes a row and lane at a time, piece 4 i + t
             float lo[4] = {}, hi[4] = {};
 #pragma unroll
             for (int i = 0; i < (int)(8 * sizeof(Code) / 4); ++i) {
-                // 16 bytes a row: pieces 4 i + t
-                const uint4 u4 = lds16(sm + Sh::piece(row, 4 * i + t)), v4 = lds16(sm + Sh::piece(row + 8, 4 * i + t));
+                const uint32_t at = ((4 * i + t) ^ sw) << 4;
+                const uint4 u4 = lds16(r0 + at), v4 = lds16(r0 + 8 * Sh::ROW + at);
                 const uint32_t u[4] = {u4.x, u4.y, u4.z, u4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
                 constexpr int PER = 16 / sizeof(Code);   // codes a piece
                 uint32_t c[PER / 2];
 #pragma unroll
                 for (int k = 0; k < PER / 8; ++k) {
-                    const uint4 w = lds16(reinterpret_cast<const uint8_t*>(s_C) + ((4 * i + t) * PER + 8 * k) * 2);
+                    const uint4 w = lds16(sm + sh.C + ((4 * i + t) * PER + 8 * k) * 2);
                     c[4 * k] = w.x; c[4 * k + 1] = w.y; c[4 * k + 2] = w.z; c[4 * k + 3] = w.w;
                 }
                 if constexpr (sizeof(Code) == 1) {
@@ -462,44 +482,37 @@ __global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateC
             }
             if (t < 2) {   // lane t = 0 has row g, t = 1 row g + 8
                 const float low = t ? lo[2] : lo[0], dot = sizeof(Code) == 1 ? low : fmaf(256.0f, t ? hi[2] : hi[0], low);
-                const uint32_t h = h0 + hh, p = row + 8 * t;
-                const uint64_t o = (uint64_t)h0 * a.P + p;
+                const uint32_t p = row + 8 * t, o = h0 * a.P + p;
                 const __half xh = *reinterpret_cast<const __half*>(sm + sh.x + n * sh.x_pitch + p * 2);
-                const float Dh = a.has_D ? __half2float(a.D[h]) : 0.0f;
-                const __half yh = __float2half_rn(fmaf(alpha * (t ? sc[1] : sc[0]), dot, (t ? dw[2] : dw[0]) * p2.down) + Dh * __half2float(xh));
+                const __half yh = __float2half_rn(fmaf(t ? as[1] : as[0], dot, t ? yw[1] : yw[0]) + s_D[hh] * __half2float(xh));
                 a.y[b * a.y_bs + o] = a.z ? __float2half_rn(silu(__half2float(a.z[b * a.z_bs + o])) * __half2float(yh)) : yh;
                 a.win_x[((uint64_t)b * a.W + n) * xrow + o] = xh;
             }
             if (!fold) continue;
         }
         // the window's part of the state: w_j x_j[p] in two f16 terms, scaled, times the window's B
-        float xw[KB * 8];
-#pragma unroll
-        for (int k = 0; k < KB; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = MODE == 0 || count ? __half22float2(bits_h2(X[k][i])) : make_float2(0.0f, 0.0f);
-                const uint32_t j = 16 * k + 2 * t + 8 * (i >> 1);
-                xw[8 * k + 2 * i] = s_w[hh][j] * f.x;
-                xw[8 * k + 2 * i + 1] = s_w[hh][j + 1] * f.y;
-            }
         const Pow2 p2(xw);
         uint32_t ah[KB][4], al[KB][4];
 #pragma unroll
         for (int k = 0; k < KB; ++k)
 #pragma unroll
             for (int i = 0; i < 4; ++i) split2(xw[8 * k + 2 * i] * p2.up, xw[8 * k + 2 * i + 1] * p2.up, &ah[k][i], &al[k][i]);
-        const float as[2] = {alpha * sc[0], alpha * sc[1]};
         // elements 16 q + 4 t .. + 3 of the state, rows g and g + 8
+        auto word_at = [&](int q) {
+            const uint32_t byte = (16 * q + 4 * t) * sizeof(Code);
+            return (((byte >> 4) ^ sw) << 4) + (byte & 15);
+        };
+        const uint32_t pair0 = 4 * (g >> 1) + (g & 1);
         auto word = [&](int q, float (&s)[2][4]) {
             float cu[4], cv[4];
-            code_values<Code>(sm + Sh::word(row, 16 * q + 4 * t), cu);
-            code_values<Code>(sm + Sh::word(row + 8, 16 * q + 4 * t), cv);
+            const uint32_t at = word_at(q);
+            code_values<Code>(r0 + at, cu);
+            code_values<Code>(r0 + 8 * Sh::ROW + at, cv);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 // column c of the product is element 16 q + 4 (c / 2) + c % 2 + 2 half: a lane gets what its codes are
                 float d[4] = {};
-                const int e = 16 * q + 4 * (g >> 1) + (g & 1) + 2 * half;
+                const int e = 16 * q + pair0 + 2 * half;
                 if (MODE == 0 || count) {
 #pragma unroll
                     for (int k = 0; k < KB; ++k) {
@@ -516,13 +529,14 @@ __global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateC
             }
         };
         if constexpr (MODE == 1) {
-#pragma unroll 2
+            const uint64_t o0 = ((uint64_t)bh0 * a.P + row) * TC_N + 4 * t;
+#pragma unroll 4
             for (int q = 0; q < 8; ++q) {
                 float s[2][4];
                 word(q, s);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const uint64_t o = (bh0 * a.P + row + 8 * r) * TC_N + 16 * q + 4 * t;
+                    const uint64_t o = o0 + 8 * TC_N * r + 16 * q;
                     if (a.state_dtype == LSSM_DT_F32)
                         __stcs(reinterpret_cast<float4*>(static_cast<float*>(a.state) + o), make_float4(s[r][0], s[r][1], s[r][2], s[r][3]));
                     else {
@@ -554,12 +568,14 @@ __global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateC
 #pragma unroll
                 for (int r = 0; r < 2; ++r) amax[r] = max_keep_nan(amax[r], __shfl_xor_sync(0xffffffffu, amax[r], o));
             const RowQuant z0(amax[0], Q), z1(amax[1], Q);
+            uint8_t* w0 = sm + row * Sh::ROW;
 #pragma unroll 1
             for (int q = 0; q < 8; ++q) {
                 float s[2][4];
                 word(q, s);
-                store_codes4(reinterpret_cast<Code*>(sm + Sh::word(row, 16 * q + 4 * t)), s[0], z0);
-                store_codes4(reinterpret_cast<Code*>(sm + Sh::word(row + 8, 16 * q + 4 * t)), s[1], z1);
+                const uint32_t at = word_at(q);
+                store_codes4(reinterpret_cast<Code*>(w0 + at), s[0], z0);
+                store_codes4(reinterpret_cast<Code*>(w0 + 8 * Sh::ROW + at), s[1], z1);
             }
             if (t == 0) {
                 scales[row] = z0.scale;
@@ -568,14 +584,14 @@ __global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateC
             __syncwarp();
             for (uint32_t i = lane; i < 16 * Sh::PIECES; i += 32) {
                 const uint32_t rr = tile * 16 + i / Sh::PIECES, q = i % Sh::PIECES;
-                *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(codes) + (uint64_t)rr * Sh::ROW + q * 16) = lds16(sm + Sh::piece(rr, q));
+                *reinterpret_cast<uint4*>(codes + rr * Sh::ROW + q * 16) = lds16(sm + Sh::piece(rr, q));
             }
         }
     }
     if (MODE == 0) {
         // the first head of a group keeps the group's B row; every head takes row n from its argument
         if (first == 0 && tid < TC_N / 8)
-            *reinterpret_cast<uint4*>(wB + n * brow + 8 * tid) = lds16(sm + sh.B + n * Sh::B_PITCH + 16 * tid);
+            *reinterpret_cast<uint4*>(wB + (uint64_t)n * brow + 8 * tid) = lds16(sm + sh.B + n * Sh::B_PITCH + 16 * tid);
         if (tid < nh) a.fill[bh0 + tid] = fold ? 0 : count;
     }
 }
@@ -588,14 +604,14 @@ cudaError_t launch_tc(const StateCacheArgs& a, uint32_t heads, cudaStream_t s) {
         if (e != cudaSuccess) return e;
     }
     const uint32_t per_group = a.H / a.G;
-    k_state_tc<Code, MODE, KB><<<a.batch * a.G * ((per_group + heads - 1) / heads), TC_THREADS, bytes, s>>>(a, heads);
+    k_state_tc<Code, MODE, KB><<<dim3((per_group + heads - 1) / heads, a.G, a.batch), TC_THREADS, bytes, s>>>(a, heads);
     return cudaGetLastError();
 }
 
 template <typename Code, int MODE>
 cudaError_t launch_cached(const StateCacheArgs& a, cudaStream_t s) {
     // rows of 128 and heads of 16 rows keep the arrays' 16-byte alignment
-    bool tc = a.N == TC_N && a.P % 16 == 0 && a.P <= TC_ROWS && aligned(a.codes, 16) && aligned(a.win_x, 16) && aligned(a.win_B, 16);
+    bool tc = a.N == TC_N && a.P % 16 == 0 && a.P <= TC_ROWS && a.G <= 65535 && a.batch <= 65535 && aligned(a.codes, 16) && aligned(a.win_x, 16) && aligned(a.win_B, 16);
     if (MODE == 0) tc = tc && aligned(a.x, 16) && aligned(a.B, 16) && aligned(a.C, 16) && a.bc_bs % 8 == 0 && a.x_bs % 8 == 0;
     else tc = tc && aligned(a.state, 16);
     if (!tc) {
