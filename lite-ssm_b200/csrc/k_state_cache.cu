@@ -216,10 +216,13 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_cached(StateCacheArgs a) {
 // codes' bytes and the latency of a short CTA.
 constexpr int TC_THREADS = 256, TC_WARPS = TC_THREADS / 32, TC_N = 128, TC_HEADS = 4;
 constexpr uint32_t TC_ROWS = 256;   // rows of 8-bit codes a CTA holds (32 KB)
+#ifndef UNR
+#define UNR 4
+#endif
 #ifndef SCC
 #define SCC 4
 #endif
-constexpr int TC_CTAS = SCC;
+constexpr int TC_CTAS = SCC, TC_UNROLL = UNR;
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -291,18 +294,20 @@ struct Pow2 {
 };
 
 // Shared memory of a CTA: the heads' codes (rows of TC_N, their 16-byte pieces exchanged by row so that neither
-// 16-byte nor 4-byte reads of 8 rows meet in a bank), the window's x (a row a token) and B, C, and the pair layout of B.
+// 16-byte nor 4-byte reads of 8 rows meet in a bank), the window's x (a row a token) and B, C,
+// S_q C of every row, and the pair layout of B.
 template <typename Code, int KB>
 struct TcShared {
     static constexpr uint32_t ROW = TC_N * sizeof(Code), PIECES = ROW / 16;
     static constexpr uint32_t B_PITCH = TC_N * 2 + 16, PAIR_PITCH = TC_N + 16;   // bytes; words
-    uint32_t x_pitch, x, B, C, pairs, total;   // bytes from the start; codes are first
+    uint32_t x_pitch, x, B, C, dot, pairs, total;   // bytes from the start; codes are first
     __host__ __device__ TcShared(uint32_t rows) {   // rows: heads * P
         x_pitch = rows * 2 + 16;
         x = rows * ROW;
         B = x + KB * 16 * x_pitch;
         C = B + KB * 16 * B_PITCH;
-        pairs = C + TC_N * 2;
+        dot = C + TC_N * 2;
+        pairs = dot + rows * 4;
         total = pairs + KB * 8 * PAIR_PITCH * 4;
     }
     static __device__ __forceinline__ uint32_t swap(uint32_t row) { return (row & 1) << 2 | (row >> 1 & 3); }
@@ -313,13 +318,14 @@ __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_c
 
 // KB: blocks of 16 window tokens (W <= 16 * KB). Grid: blocks of heads, groups, sequences.
 template <typename Code, int MODE, int KB>
-__global__ void __launch_bounds__(TC_THREADS, TC_CTAS) k_state_tc(StateCacheArgs a, uint32_t heads) {
+__global__ void __launch_bounds__(TC_THREADS, TC_CTAS) k_state_tc(StateCacheArgs a, uint32_t heads, uint32_t per_group) {
     constexpr float Q = sizeof(Code) == 1 ? 127.0f : 32767.0f;
     using Sh = TcShared<Code, KB>;
     extern __shared__ __align__(128) uint8_t sm[];
-    __shared__ __align__(8) float s_w[TC_HEADS][32];
+    __shared__ __align__(16) float s_w[TC_HEADS][32];
+    __shared__ __align__(16) float s_cb[MODE == 0 ? 16 * KB : 1];
     __shared__ float s_alpha[TC_HEADS], s_D[TC_HEADS];
-    const uint32_t per_group = a.H / a.G, first = blockIdx.x * heads, nh = min(heads, per_group - first), b = blockIdx.z;
+    const uint32_t first = blockIdx.x * heads, nh = min(heads, per_group - first), b = blockIdx.z;
     const uint32_t h0 = blockIdx.y * per_group + first;   // heads h0 .. h0 + nh - 1
     const uint32_t tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t rows = nh * a.P, bh0 = b * a.H + h0;
@@ -335,19 +341,20 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) k_state_tc(StateCacheArgs
         uint32_t to = sm0 + Sh::piece(tid / Sh::PIECES, tid % Sh::PIECES);
         for (uint32_t r = tid / Sh::PIECES; r < rows; r += STEP, from += TC_THREADS * 16, to += TC_THREADS * 16) copy_async16(to, from);
     }
-    // what warp w < nh needs for head w's weights; scales of this warp's first tile
-    float p_dt = 0.0f, p_raw = 0.0f, p_bias = 0.0f, p_A = 0.0f, p_D = 0.0f, sc[2] = {};
+    // what warp w < nh needs for head w's weights, and this thread's row
+    float p_dt = 0.0f;
+    __half p_raw = __ushort_as_half(0), p_bias = p_raw, p_A = p_raw, p_D = p_raw;
     if (wid < nh) {
         const uint32_t h = h0 + wid;
         if (lane < a.W) p_dt = a.win_dt[(uint64_t)(bh0 + wid) * a.W + lane];
-        p_A = __half2float(a.A_log[h]);
+        p_A = a.A_log[h];
         if (MODE == 0) {
-            p_raw = __half2float(a.dt_raw[b * a.dt_bs + h]);
-            p_bias = __half2float(a.dt_bias[h]);
-            if (a.has_D) p_D = __half2float(a.D[h]);
+            p_raw = a.dt_raw[b * a.dt_bs + h];
+            p_bias = a.dt_bias[h];
+            if (a.has_D) p_D = a.D[h];
         }
     }
-    if (wid < rows / 16) { sc[0] = scales[wid * 16 + g]; sc[1] = scales[wid * 16 + g + 8]; }
+    const float my_scale = tid < rows ? scales[tid] : 0.0f;
     // A step's token is number n of the window; `count` tokens with it. All heads of a sequence have the same.
     const uint32_t n = MODE == 0 ? min(filled, a.W - 1) : a.W, count = MODE == 0 ? n + 1 : min(filled, a.W);
     const bool fold = MODE == 0 && count == a.W;
@@ -376,11 +383,11 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) k_state_tc(StateCacheArgs
     if (MODE == 0 && tid < TC_N / 8) copy_async16(sm0 + sh.C + tid * 16, a.C + b * a.bc_bs + blockIdx.y * TC_N + tid * 8);
     if (wid < nh) {
         float dt = lane < count ? p_dt : 0.0f;
-        if (MODE == 0 && lane == n) dt = token_dt(p_raw + p_bias, a.dt_min, a.dt_max);
+        if (MODE == 0 && lane == n) dt = token_dt(__half2float(p_raw) + __half2float(p_bias), a.dt_min, a.dt_max);
         float wj, al;
-        window_weights(-expf(p_A), dt, lane, count, &wj, &al);
+        window_weights(-expf(__half2float(p_A)), dt, lane, count, &wj, &al);
         s_w[wid][lane] = wj;
-        if (lane == 0) { s_alpha[wid] = al; s_D[wid] = p_D; }
+        if (lane == 0) { s_alpha[wid] = al; s_D[wid] = __half2float(p_D); }
         if (MODE == 0 && lane == n) a.win_dt[(uint64_t)(bh0 + wid) * a.W + n] = dt;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -395,60 +402,17 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) k_state_tc(StateCacheArgs
             const uint32_t p0 = *reinterpret_cast<const uint32_t*>(from), p1 = *reinterpret_cast<const uint32_t*>(from + Sh::B_PITCH);
             *reinterpret_cast<uint2*>(&pairs[jp][e]) = make_uint2(__byte_perm(p0, p1, 0x5410), __byte_perm(p0, p1, 0x7632));
         }
-        __syncthreads();
+        if (MODE == 1) __syncthreads();
     }
-    // C . B_j in every warp: rows j = g and g + 8 of every block, then to the lanes that use them: tokens
-    // 16 k + {2t, 2t + 1, 2t + 8, 2t + 9}
-    float cb[KB][4];
+    auto head_of = [&](uint32_t row) { return (uint32_t)(row >= a.P) + (row >= 2 * a.P) + (row >= 3 * a.P); };
     if constexpr (MODE == 0) {
-#pragma unroll
-        for (int k = 0; k < KB; ++k) {
-            float d[4] = {};
-            const uint8_t* r0 = sm + sh.B + (16 * k + g) * Sh::B_PITCH + 16 * t;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint4 p0 = lds16(r0 + 64 * i), p1 = lds16(r0 + 8 * Sh::B_PITCH + 64 * i), c = lds16(sm + sh.C + 64 * i + 16 * t);
-                mma16816(d, p0.x, p1.x, p0.y, p1.y, c.x, c.y);
-                mma16816(d, p0.z, p1.z, p0.w, p1.w, c.z, c.w);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) cb[k][i] = __shfl_sync(0xffffffffu, d[i & 2], 8 * t + 4 * (i & 1));
-        }
-    }
-    const uint32_t ldm = sm0 + sh.x + ((lane & 7) + (lane >> 4 & 1) * 8) * sh.x_pitch + (lane >> 3 & 1) * 16;
-    for (uint32_t tile = wid; tile < rows / 16; tile += TC_WARPS) {
-        const uint32_t row = tile * 16 + g, hh = tile * 16 / a.P;   // rows of the CTA's heads
-        const float alpha = s_alpha[hh];
-        if (tile != wid) { sc[0] = scales[row]; sc[1] = scales[row + 8]; }
-        const float as[2] = {alpha * sc[0], alpha * sc[1]};
-        // w_j x_j[p] of the lane's tokens: [0], [1] row g, tokens 2t, 2t + 1; [2], [3] row g + 8; [4] .. [7] tokens + 8
-        float xw[KB * 8];
-#pragma unroll
-        for (int k = 0; k < KB; ++k) {
-            uint32_t X[4] = {};
-            if (MODE == 0 || count) ldmatrix_t(X, ldm + 16 * k * sh.x_pitch + tile * 32);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = __half22float2(bits_h2(X[i])), w = *reinterpret_cast<const float2*>(&s_w[hh][16 * k + 2 * t + 8 * (i >> 1)]);
-                xw[8 * k + 2 * i] = w.x * f.x;
-                xw[8 * k + 2 * i + 1] = w.y * f.y;
-            }
-        }
-        const uint32_t sw = Sh::swap(row);   // of row + 8, too
-        const uint8_t* r0 = sm + row * Sh::ROW;
-        if constexpr (MODE == 0) {
-            float yw[2] = {};
-#pragma unroll
-            for (int k = 0; k < KB; ++k)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) yw[i >> 1 & 1] = fmaf(xw[8 * k + i], cb[k][(i & 1) + 2 * (i >> 2)], yw[i >> 1 & 1]);
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                yw[r] += __shfl_xor_sync(0xffffffffu, yw[r], 1);
-                yw[r] += __shfl_xor_sync(0xffffffffu, yw[r], 2);
-            }
-            // S_q C: 16 bytes a row and lane at a time, piece 4 i + t
-            float lo[4] = {}, hi[4] = {};
+        float* s_dot = reinterpret_cast<float*>(sm + sh.dot);
+        // S_q C of every row
+        for (uint32_t tile = wid; tile < rows / 16; tile += TC_WARPS) {
+            const uint32_t row = tile * 16 + g, sw = Sh::swap(row);   // of row + 8, too
+            const uint8_t* r0 = sm + row * Sh::ROW;
+            // 16 bytes a row and lane at a time, piece 4 i + t
+            float lo[2][4] = {}, hi[2][4] = {};
 #pragma unroll
             for (int i = 0; i < (int)(8 * sizeof(Code) / 4); ++i) {
                 const uint32_t at = ((4 * i + t) ^ sw) << 4;
@@ -465,30 +429,88 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) k_state_tc(StateCacheArgs
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const uint32_t x = u[q] ^ 0x80808080u, y = v[q] ^ 0x80808080u;
-                        mma16816(lo, bytes_h2(x, 0x4140, 1152.0f), bytes_h2(y, 0x4140, 1152.0f), bytes_h2(x, 0x4342, 1152.0f),
+                        mma16816(lo[q & 1], bytes_h2(x, 0x4140, 1152.0f), bytes_h2(y, 0x4140, 1152.0f), bytes_h2(x, 0x4342, 1152.0f),
                                  bytes_h2(y, 0x4342, 1152.0f), c[2 * q], c[2 * q + 1]);
                     }
                 } else {
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         const uint32_t x0 = u[2 * q], x1 = u[2 * q + 1], y0 = v[2 * q], y1 = v[2 * q + 1];
-                        mma16816(lo, bytes_h2(x0, 0x4240, 1024.0f), bytes_h2(y0, 0x4240, 1024.0f), bytes_h2(x1, 0x4240, 1024.0f),
+                        mma16816(lo[q], bytes_h2(x0, 0x4240, 1024.0f), bytes_h2(y0, 0x4240, 1024.0f), bytes_h2(x1, 0x4240, 1024.0f),
                                  bytes_h2(y1, 0x4240, 1024.0f), c[2 * q], c[2 * q + 1]);
-                        mma16816(hi, bytes_h2(x0 ^ 0x80008000u, 0x4341, 1152.0f), bytes_h2(y0 ^ 0x80008000u, 0x4341, 1152.0f),
+                        mma16816(hi[q], bytes_h2(x0 ^ 0x80008000u, 0x4341, 1152.0f), bytes_h2(y0 ^ 0x80008000u, 0x4341, 1152.0f),
                                  bytes_h2(x1 ^ 0x80008000u, 0x4341, 1152.0f), bytes_h2(y1 ^ 0x80008000u, 0x4341, 1152.0f), c[2 * q],
                                  c[2 * q + 1]);
                     }
                 }
             }
-            if (t < 2) {   // lane t = 0 has row g, t = 1 row g + 8
-                const float low = t ? lo[2] : lo[0], dot = sizeof(Code) == 1 ? low : fmaf(256.0f, t ? hi[2] : hi[0], low);
-                const uint32_t p = row + 8 * t, o = h0 * a.P + p;
-                const __half xh = *reinterpret_cast<const __half*>(sm + sh.x + n * sh.x_pitch + p * 2);
-                const __half yh = __float2half_rn(fmaf(t ? as[1] : as[0], dot, t ? yw[1] : yw[0]) + s_D[hh] * __half2float(xh));
-                a.y[b * a.y_bs + o] = a.z ? __float2half_rn(silu(__half2float(a.z[b * a.z_bs + o])) * __half2float(yh)) : yh;
-                a.win_x[((uint64_t)b * a.W + n) * xrow + o] = xh;
+            if (t < 2) {   // every column has the dot; lane t = 0 stores row g, t = 1 row g + 8
+                const float l = t ? lo[0][2] + lo[1][2] : lo[0][0] + lo[1][0], h = t ? hi[0][2] + hi[1][2] : hi[0][0] + hi[1][0];
+                s_dot[row + 8 * t] = sizeof(Code) == 1 ? l : fmaf(256.0f, h, l);
             }
-            if (!fold) continue;
+        }
+        // C . B_j of the window's tokens: 16 a warp, from the last warp on
+        if (wid >= TC_WARPS - KB) {
+            float d[4] = {};
+            const uint32_t j0 = 16 * (TC_WARPS - 1 - wid) + g;
+            const uint8_t* r0 = sm + sh.B + j0 * Sh::B_PITCH + 16 * t;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4 p0 = lds16(r0 + 64 * i), p1 = lds16(r0 + 8 * Sh::B_PITCH + 64 * i), c = lds16(sm + sh.C + 64 * i + 16 * t);
+                mma16816(d, p0.x, p1.x, p0.y, p1.y, c.x, c.y);
+                mma16816(d, p0.z, p1.z, p0.w, p1.w, c.z, c.w);
+            }
+            if (t == 0) { s_cb[j0] = d[0]; s_cb[j0 + 8] = d[2]; }
+        }
+        __syncthreads();
+        // y: a thread a row
+        if (tid < rows) {
+            const uint32_t hh = head_of(tid);
+            const __half* x = reinterpret_cast<const __half*>(sm + sh.x) + tid;
+            const float* w = s_w[hh];
+            float yw = 0.0f;
+#pragma unroll
+            for (uint32_t j0 = 0; j0 < 16 * KB; j0 += 4) {
+                if (j0 >= count) break;   // a token behind the window's has weight 0 and x 0
+                const float4 c4 = *reinterpret_cast<const float4*>(&s_cb[j0]), w4 = *reinterpret_cast<const float4*>(&w[j0]);
+                const float cw[4] = {c4.x * w4.x, c4.y * w4.y, c4.z * w4.z, c4.w * w4.w};
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                    yw = fmaf(cw[j], __half2float(*reinterpret_cast<const __half*>(reinterpret_cast<const uint8_t*>(x) + (j0 + j) * sh.x_pitch)), yw);
+            }
+            const __half xh = *reinterpret_cast<const __half*>(reinterpret_cast<const uint8_t*>(x) + n * sh.x_pitch);
+            const __half yh = __float2half_rn(fmaf(s_alpha[hh] * my_scale, s_dot[tid], yw) + s_D[hh] * __half2float(xh));
+            const uint32_t o = h0 * a.P + tid;
+            a.y[b * a.y_bs + o] = a.z ? __float2half_rn(silu(__half2float(a.z[b * a.z_bs + o])) * __half2float(yh)) : yh;
+            a.win_x[((uint64_t)b * a.W + n) * xrow + o] = xh;
+        }
+        // the first head of a group keeps the group's B row; every head takes row n from its argument
+        if (first == 0 && tid < TC_N / 8)
+            *reinterpret_cast<uint4*>(wB + (uint64_t)n * brow + 8 * tid) = lds16(sm + sh.B + n * Sh::B_PITCH + 16 * tid);
+        if (tid < nh) a.fill[bh0 + tid] = fold ? 0 : count;
+        if (!fold) return;
+    }
+    float* s_as = reinterpret_cast<float*>(sm + sh.dot);   // alpha * scale of every row
+    if (MODE == 0) __syncthreads();
+    if (tid < rows) s_as[tid] = s_alpha[head_of(tid)] * my_scale;
+    __syncthreads();
+    const uint32_t ldm = sm0 + sh.x + ((lane & 7) + (lane >> 4 & 1) * 8) * sh.x_pitch + (lane >> 3 & 1) * 16;
+    for (uint32_t tile = wid; tile < rows / 16; tile += TC_WARPS) {
+        const uint32_t row = tile * 16 + g, hh = head_of(tile * 16), sw = Sh::swap(row);   // of row + 8, too
+        const uint8_t* r0 = sm + row * Sh::ROW;
+        const float as[2] = {s_as[row], s_as[row + 8]};
+        // w_j x_j[p] of the lane's tokens: [0], [1] row g, tokens 2t, 2t + 1; [2], [3] row g + 8; [4] .. [7] tokens + 8
+        float xw[KB * 8];
+#pragma unroll
+        for (int k = 0; k < KB; ++k) {
+            uint32_t X[4] = {};
+            if (MODE == 0 || count) ldmatrix_t(X, ldm + 16 * k * sh.x_pitch + tile * 32);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = __half22float2(bits_h2(X[i])), w = *reinterpret_cast<const float2*>(&s_w[hh][16 * k + 2 * t + 8 * (i >> 1)]);
+                xw[8 * k + 2 * i] = w.x * f.x;
+                xw[8 * k + 2 * i + 1] = w.y * f.y;
+            }
         }
         // the window's part of the state: w_j x_j[p] in two f16 terms, scaled, times the window's B
         const Pow2 p2(xw);
@@ -530,7 +552,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) k_state_tc(StateCacheArgs
         };
         if constexpr (MODE == 1) {
             const uint64_t o0 = ((uint64_t)bh0 * a.P + row) * TC_N + 4 * t;
-#pragma unroll 4
+#pragma unroll TC_UNROLL
             for (int q = 0; q < 8; ++q) {
                 float s[2][4];
                 word(q, s);
@@ -588,12 +610,6 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) k_state_tc(StateCacheArgs
             }
         }
     }
-    if (MODE == 0) {
-        // the first head of a group keeps the group's B row; every head takes row n from its argument
-        if (first == 0 && tid < TC_N / 8)
-            *reinterpret_cast<uint4*>(wB + (uint64_t)n * brow + 8 * tid) = lds16(sm + sh.B + n * Sh::B_PITCH + 16 * tid);
-        if (tid < nh) a.fill[bh0 + tid] = fold ? 0 : count;
-    }
 }
 
 template <typename Code, int MODE, int KB>
@@ -604,7 +620,7 @@ cudaError_t launch_tc(const StateCacheArgs& a, uint32_t heads, cudaStream_t s) {
         if (e != cudaSuccess) return e;
     }
     const uint32_t per_group = a.H / a.G;
-    k_state_tc<Code, MODE, KB><<<dim3((per_group + heads - 1) / heads, a.G, a.batch), TC_THREADS, bytes, s>>>(a, heads);
+    k_state_tc<Code, MODE, KB><<<dim3((per_group + heads - 1) / heads, a.G, a.batch), TC_THREADS, bytes, s>>>(a, heads, per_group);
     return cudaGetLastError();
 }
 
