@@ -41,6 +41,15 @@ struct RowQuant {
         inv = scale > 0.0f ? __frcp_rn(scale) : 0.0f;
         half = scale > 0.0f ? 0.5f * scale : INFINITY;
     }
+    // what lane l of the warp has
+    __device__ __forceinline__ RowQuant of_lane(int l) const {
+        RowQuant z = *this;
+        z.scale = __shfl_sync(0xffffffffu, scale, l);
+        z.inv = __shfl_sync(0xffffffffu, inv, l);
+        z.half = z.scale > 0.0f ? 0.5f * z.scale : INFINITY;
+        z.sound = z.scale == z.scale;
+        return z;
+    }
 };
 // Codes of four elements as whole numbers in the low bits of the results. Added to 1.5 * 2^23, v / scale is rounded
 // to a whole number, ties to even, but the reciprocal may have carried it over a half step. The remainder
@@ -216,13 +225,6 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_cached(StateCacheArgs a) {
 // codes' bytes and the latency of a short CTA.
 constexpr int TC_THREADS = 256, TC_WARPS = TC_THREADS / 32, TC_N = 128, TC_HEADS = 4;
 constexpr uint32_t TC_ROWS = 256;   // rows of 8-bit codes a CTA holds (32 KB)
-#ifndef UNR
-#define UNR 4
-#endif
-#ifndef SCC
-#define SCC 4
-#endif
-constexpr int TC_CTAS = SCC, TC_UNROLL = UNR;
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -318,7 +320,7 @@ __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_c
 
 // KB: blocks of 16 window tokens (W <= 16 * KB). Grid: blocks of heads, groups, sequences.
 template <typename Code, int MODE, int KB>
-__global__ void __launch_bounds__(TC_THREADS, TC_CTAS) k_state_tc(StateCacheArgs a, uint32_t heads, uint32_t per_group) {
+__global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_state_tc(StateCacheArgs a, uint32_t heads, uint32_t per_group) {
     constexpr float Q = sizeof(Code) == 1 ? 127.0f : 32767.0f;
     using Sh = TcShared<Code, KB>;
     extern __shared__ __align__(128) uint8_t sm[];
@@ -552,7 +554,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) k_state_tc(StateCacheArgs
         };
         if constexpr (MODE == 1) {
             const uint64_t o0 = ((uint64_t)bh0 * a.P + row) * TC_N + 4 * t;
-#pragma unroll TC_UNROLL
+#pragma unroll
             for (int q = 0; q < 8; ++q) {
                 float s[2][4];
                 word(q, s);
@@ -578,7 +580,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) k_state_tc(StateCacheArgs
             // The rows' largest elements first, then the codes: computed twice, once in W steps, so that no step
             // holds the registers for it.
             float amax[2] = {};
-#pragma unroll 1
+#pragma unroll
             for (int q = 0; q < 8; ++q) {
                 float s[2][4];
                 word(q, s);
@@ -591,7 +593,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) k_state_tc(StateCacheArgs
                 for (int r = 0; r < 2; ++r) amax[r] = max_keep_nan(amax[r], __shfl_xor_sync(0xffffffffu, amax[r], o));
             const RowQuant z0(amax[0], Q), z1(amax[1], Q);
             uint8_t* w0 = sm + row * Sh::ROW;
-#pragma unroll 1
+#pragma unroll
             for (int q = 0; q < 8; ++q) {
                 float s[2][4];
                 word(q, s);
@@ -640,9 +642,6 @@ cudaError_t launch_cached(const StateCacheArgs& a, cudaStream_t s) {
     uint32_t heads = TC_HEADS;
     while (heads > 1 && (heads * a.P > TC_ROWS / sizeof(Code) ||
                          (uint64_t)a.batch * a.G * ((per_group + heads - 1) / heads) < 2ull * 148)) heads /= 2;
-#ifdef SCENV
-    if (getenv("SC_HEADS")) heads = atoi(getenv("SC_HEADS"));
-#endif
     return a.W <= 16 ? launch_tc<Code, MODE, 1>(a, heads, s) : launch_tc<Code, MODE, 2>(a, heads, s);
 }
 
@@ -678,19 +677,29 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_store128(StateCacheArgs a)
 #pragma unroll
     for (int r = 0; r < STORE_ROWS; ++r)
         if (row0 + r < rows) v[r] = __ldcs(reinterpret_cast<const float4*>(S + r * 128));
+    // lane r works out row r's scale
+    uint32_t mine = 0;
+#pragma unroll
+    for (int r = 0; r < STORE_ROWS; ++r) {
+        uint32_t top = 0;
+        if (row0 + r < rows) {
+            const float e[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(e[i]) & 0x7FFFFFFFu);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if ((int)lane == r) mine = top;
+    }
+    const RowQuant own(__uint_as_float(mine), Q);
 #pragma unroll
     for (int r = 0; r < STORE_ROWS; ++r) {
         if (row0 + r >= rows) break;
         const float e[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(e[i]) & 0x7FFFFFFFu);
-        const RowQuant z(__uint_as_float(__reduce_max_sync(0xffffffffu, top)), Q);
-        store_codes4(out + r * 128, e, z);
-        if (lane == 0) {
-            a.scales[row0 + r] = z.scale;
-            if ((row0 + r) % a.P == 0) a.fill[(row0 + r) / a.P] = 0;
-        }
+        store_codes4(out + r * 128, e, own.of_lane(r));
+    }
+    if (lane < STORE_ROWS && row0 + lane < rows) {
+        a.scales[row0 + lane] = own.scale;
+        if ((row0 + lane) % a.P == 0) a.fill[(row0 + lane) / a.P] = 0;
     }
 }
 
