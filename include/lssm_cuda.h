@@ -377,6 +377,19 @@ lssm_status lssm_generate(lssm_session* s, const uint32_t* prompt, uint32_t L, u
                           uint32_t eos, uint32_t* out_tokens, uint32_t* n_out);
 /* fp32 copy of the logits of the last position computed (batch x vocab, host). */
 lssm_status lssm_session_logits(lssm_session* s, float* out);
+/* Scores L tokens per sequence (tokens: batch x L, host) as a continuation of the session's state: a
+ * prefill that keeps every position's distribution. Entry i of a sequence's L outputs (host, batch x L;
+ * top_ids / top_logp batch x L x top_k) is lssm_logprobs of the logits after token i with token i + 1 as
+ * the target; the last entry's logp is 0 (no target). -mean(logp[:-1]) is the mean negative log
+ * likelihood, its exponential the perplexity. Any output may be null, but not all. Afterwards the session
+ * is where lssm_prefill of the same tokens leaves it. Not for tensor-parallel sessions (LSSM_ERR_STATE). */
+lssm_status lssm_score(lssm_session* s, const uint32_t* tokens, uint32_t L, uint32_t top_k, float* logp,
+                       float* entropy, uint32_t* top_ids, float* top_logp);
+/* lssm_logprobs of the logits of the last position computed, one row per sequence (host arrays of batch,
+ * batch x top_k): what a decode step's token was worth, and its alternatives. targets: batch ids, or null
+ * without logp. Not for tensor-parallel sessions (LSSM_ERR_STATE). */
+lssm_status lssm_session_logprobs(lssm_session* s, const uint32_t* targets, uint32_t top_k, float* logp,
+                                  float* entropy, uint32_t* top_ids, float* top_logp);
 /* Device timing of the last prefill / decode call (CUDA events on the session stream), ms. */
 lssm_status lssm_session_timing(lssm_session* s, float* prefill_ms, float* decode_ms);
 /* Kernel launches issued by the last prefill and by the last lssm_decode call (all its
@@ -387,6 +400,12 @@ lssm_status lssm_session_launches(lssm_session* s, uint64_t* prefill, uint64_t* 
  *                qualifies (batch <= 2, INT4_B32 in/out_proj, fp16 lm_head, d_state 128,
  *                d_model and d_inner multiples of 256) (default 1);
  *   "cuda_graph" 1 = otherwise capture each decode step in a CUDA graph (default 1);
+ *   "state_bits" 8 or 16 = decode over a quantised state cache (lssm_ssd_step_cached) where the
+ *                persistent kernel does not run: the states move from fp32 to the cache at the
+ *                first decode after a prefill, and back before the next prefill or persistent
+ *                decode. 0 = fp32 states (default). Needs memory of its own besides the fp32
+ *                states (which the prefill scan keeps).
+ *   "state_window" tokens between two roundings of the cached states, 1..32 (default 16)
  *   "trace"      1 = record per-phase %globaltimer stamps of the persistent kernel's first
  *                step (read with lssm_session_trace). */
 lssm_status lssm_session_set_option(lssm_session* s, const char* key, int64_t value);

@@ -576,6 +576,14 @@ struct lssm_session {
     // greedy pick: per-chunk (value, index) pairs, per-row tickets, per-rank row pairs
     uint2 *d_cpair = nullptr, *d_pair = nullptr;
     uint32_t* d_ticket = nullptr;
+    // quantised states of the per-op decode (option "state_bits"): one block with every layer's cache. While
+    // `in_cache`, the states are there and `ssd` is stale.
+    uint32_t state_bits = 0, state_window = 16;
+    bool in_cache = false;
+    uint8_t* d_cache = nullptr;
+    // scoring: logits of a run of rows, targets, results (grown on demand)
+    uint8_t* d_score = nullptr;
+    size_t score_bytes = 0;
 };
 
 static lssm_status s_alloc(void** p, size_t n, const char* what) {
@@ -592,7 +600,7 @@ extern "C" lssm_status lssm_session_destroy(lssm_session* s) {
     void* ps[] = {s->conv, s->ssd, s->hidden, s->normed, s->proj, s->xs, s->Bs, s->Cs, s->ys, s->gated, s->mixn,
                   s->logits, s->lastrows, s->wscratch, s->d_tokens, s->d_cur, s->d_hist, s->d_step, s->d_err,
                   s->d_players, s->d_part_val, s->d_part_idx, s->d_bar, s->d_trace, s->d_maps, s->d_opart, s->d_mb,
-                  s->d_shard, s->d_sumsq, s->d_part32, s->d_gather, s->d_cpair, s->d_pair, s->d_ticket};
+                  s->d_shard, s->d_sumsq, s->d_part32, s->d_gather, s->d_cpair, s->d_pair, s->d_ticket, s->d_cache, s->d_score};
     for (void* p : ps)
         if (p) cudaFree(p);
     for (auto& e : s->ev)
@@ -967,6 +975,77 @@ extern "C" lssm_status lssm_session_reset(lssm_session* s) {
     if (e == cudaSuccess) e = cudaStreamSynchronize(s->ctx->stream);
     if (e != cudaSuccess) return cuda_fail(e, "Mamba2State::reset");
     s->logits_valid = false;
+    s->in_cache = false;
+    return LSSM_OK;
+}
+
+#define CU(expr)                                                  \
+    do {                                                          \
+        cudaError_t _e = (expr);                                  \
+        if (_e != cudaSuccess) return cuda_fail(_e, #expr);       \
+    } while (0)
+
+// ---- quantised states (k_state_cache.cu) ----------------------------------------
+static size_t cache_layer_bytes(const lssm_session* s, uint32_t bits, size_t* off) {
+    const SsmHeader& h = s->m->img.hdr;
+    lssm_state_cache_dims d{};
+    d.batch = s->batch; d.H = s->H; d.P = h.d_head; d.N = h.d_state; d.n_groups = s->G;
+    d.window = s->state_window; d.bits = bits;
+    uint64_t n[6];
+    if (lssm_state_cache_bytes(d, n)) return 0;   // the shape is beyond the cache's limits
+    size_t at = 0;
+    for (int i = 0; i < 6; ++i) {
+        if (off) off[i] = at;
+        at += al256(n[i]);
+    }
+    return at;
+}
+static StateCacheArgs cache_args(const lssm_session* s, uint32_t layer) {
+    const SsmHeader& h = s->m->img.hdr;
+    size_t off[6];
+    uint8_t* base = s->d_cache + cache_layer_bytes(s, s->state_bits, off) * layer;
+    StateCacheArgs a{};
+    a.codes = base + off[0];
+    a.scales = reinterpret_cast<float*>(base + off[1]);
+    a.win_x = reinterpret_cast<__half*>(base + off[2]);
+    a.win_B = reinterpret_cast<__half*>(base + off[3]);
+    a.win_dt = reinterpret_cast<float*>(base + off[4]);
+    a.fill = reinterpret_cast<uint32_t*>(base + off[5]);
+    a.A_log = s->lw[layer].A_log;
+    a.state = s->ssd + s->ssd_layer * layer;
+    a.state_dtype = LSSM_DT_F32;
+    a.batch = s->batch; a.H = s->H; a.P = h.d_head; a.N = h.d_state; a.G = s->G;
+    a.W = s->state_window; a.bits = s->state_bits;
+    a.dt_min = 1e-6f; a.dt_max = 1e6f; a.has_D = 1;
+    return a;
+}
+// The states to where the next call wants them: the cache (per-op decode under "state_bits") or fp32.
+static lssm_status states_to(lssm_session* s, bool cache, cudaStream_t st) {
+    if (s->in_cache == cache) return LSSM_OK;
+    for (uint32_t l = 0; l < s->m->img.hdr.n_layer; ++l) {
+        const StateCacheArgs a = cache_args(s, l);
+        CU(cache ? launch_state_store(a, st) : launch_state_load(a, st));
+        s->nl += 1;
+    }
+    s->in_cache = cache;
+    return LSSM_OK;
+}
+static lssm_status set_state_cache(lssm_session* s, uint32_t bits, uint32_t window) {
+    if (bits == s->state_bits && window == s->state_window) return LSSM_OK;
+    if (lssm_status r = states_to(s, false, s->ctx->stream)) return r;
+    CU(cudaStreamSynchronize(s->ctx->stream));
+    if (s->graph) { cudaGraphExecDestroy(s->graph); s->graph = nullptr; }
+    if (s->d_cache) { cudaFree(s->d_cache); s->d_cache = nullptr; }
+    s->state_window = window;
+    s->state_bits = 0;   // until the memory is there
+    if (!bits) return LSSM_OK;
+    const size_t layer = cache_layer_bytes(s, bits, nullptr);
+    if (!layer) return fail(LSSM_ERR_INVALID_ARGUMENT, "lssm_session_set_option: the model's shape has no state cache");
+    if (lssm_status r = s_alloc(reinterpret_cast<void**>(&s->d_cache), layer * s->m->img.hdr.n_layer, "session: state cache"))
+        return r;
+    // windows are read up to their fill only; the rest stays zero
+    CU(cudaMemsetAsync(s->d_cache, 0, layer * s->m->img.hdr.n_layer, s->ctx->stream));
+    s->state_bits = bits;
     return LSSM_OK;
 }
 
@@ -990,6 +1069,18 @@ extern "C" lssm_status lssm_session_set_option(lssm_session* s, const char* key,
         if (s->graph) { cudaGraphExecDestroy(s->graph); s->graph = nullptr; }
         return LSSM_OK;
     }
+    if (std::strcmp(key, "state_bits") == 0) {
+        if (value != 0 && value != 8 && value != 16)
+            return fail(LSSM_ERR_INVALID_ARGUMENT, "lssm_session_set_option: state_bits must be 0, 8 or 16");
+        cudaSetDevice(s->ctx->device);
+        return set_state_cache(s, (uint32_t)value, s->state_window);
+    }
+    if (std::strcmp(key, "state_window") == 0) {
+        if (value < 1 || value > (int64_t)LSSM_STATE_WINDOW_MAX)
+            return fail(LSSM_ERR_INVALID_ARGUMENT, "lssm_session_set_option: state_window must be 1..%u", LSSM_STATE_WINDOW_MAX);
+        cudaSetDevice(s->ctx->device);
+        return set_state_cache(s, s->state_bits, (uint32_t)value);
+    }
     if (std::strcmp(key, "tp_p2p") == 0) {   // set alike on every rank
         s->use_p2p = value != 0;
         if (s->graph) { cudaGraphExecDestroy(s->graph); s->graph = nullptr; }
@@ -997,12 +1088,6 @@ extern "C" lssm_status lssm_session_set_option(lssm_session* s, const char* key,
     }
     return fail(LSSM_ERR_INVALID_ARGUMENT, "lssm_session_set_option: unknown key '%s'", key);
 }
-
-#define CU(expr)                                                  \
-    do {                                                          \
-        cudaError_t _e = (expr);                                  \
-        if (_e != cudaSuccess) return cuda_fail(_e, #expr);       \
-    } while (0)
 
 static inline const void* W(const lssm_model* m, const TensorRec* t) { return m->d_base + t->offset; }
 
@@ -1077,7 +1162,15 @@ static lssm_status run_block(lssm_session* s, uint32_t layer, uint32_t L, bool d
         a.batch = B; a.H = H; a.P = P; a.N = N; a.G = s->G;
         a.dt_min = 1e-6f; a.dt_max = 1e6f; a.has_D = 1;
         a.x_bs = di; a.bc_bs = GN; a.dt_bs = proj; a.y_bs = di; a.z_bs = proj;
-        CU(launch_ssd_step_ex(a, st));
+        if (s->in_cache) {
+            StateCacheArgs c = cache_args(s, layer);
+            c.x = a.x; c.B = a.B; c.C = a.C; c.dt_raw = a.dt_raw; c.dt_bias = a.dt_bias; c.D = a.D;
+            c.y = a.y; c.z = a.z;
+            c.x_bs = a.x_bs; c.bc_bs = a.bc_bs; c.dt_bs = a.dt_bs; c.y_bs = a.y_bs; c.z_bs = a.z_bs;
+            CU(launch_ssd_step_cached(c, st));
+        } else {
+            CU(launch_ssd_step_ex(a, st));
+        }
         s->nl += 2;
     } else {
         CU(launch_conv_silu_split(xbc, proj, lw.conv_w, lw.conv_b, s->xs, s->Bs, s->Cs, B, L, di, GN, Kc, st));
@@ -1172,17 +1265,13 @@ static lssm_status check_err(lssm_session* s, const char* what) {
     return LSSM_OK;
 }
 
-extern "C" lssm_status lssm_prefill(lssm_session* s, const uint32_t* tokens, uint32_t L, uint32_t* next_tokens) {
-    if (!s || !tokens) return fail(LSSM_ERR_INVALID_ARGUMENT, "lssm_prefill: null argument");
-    if (L == 0) return fail(LSSM_ERR_INVALID_ARGUMENT, "forward_prefill: L must be >= 1");
-    if (L > s->max_L) return fail(LSSM_ERR_INVALID_ARGUMENT, "forward_prefill: L exceeds workspace max_seq_len");
-    cudaSetDevice(s->ctx->device);
-    cudaStream_t st = s->ctx->stream;
+// tokens (batch x L, host) through all layers: hidden rows, states. From the event ev[0] on.
+static lssm_status forward_rows(lssm_session* s, const uint32_t* tokens, uint32_t L, cudaStream_t st) {
     lssm_model* m = s->m;
     const SsmHeader& h = m->img.hdr;
     const uint32_t rows = s->batch * L;
+    if (lssm_status r = states_to(s, false, st)) return r;
     CU(cudaMemcpyAsync(s->d_tokens, tokens, (size_t)rows * 4, cudaMemcpyHostToDevice, st));
-    const uint64_t nl0 = s->nl;
     CU(cudaEventRecord(s->ev[0], st));   // device timing starts with the tokens resident in HBM
     CU(launch_embed_gather(s->d_tokens, W(m, m->embed), s->hidden, rows, h.d_model, h.vocab_size, s->d_err, st));
     s->nl += 1;
@@ -1191,6 +1280,17 @@ extern "C" lssm_status lssm_prefill(lssm_session* s, const uint32_t* tokens, uin
     // last row of each sequence -> contiguous (batch, d_model)
     CU(cudaMemcpy2DAsync(s->lastrows, (size_t)h.d_model * 2, s->hidden + (size_t)(L - 1) * h.d_model,
                          (size_t)L * h.d_model * 2, (size_t)h.d_model * 2, s->batch, cudaMemcpyDeviceToDevice, st));
+    return LSSM_OK;
+}
+
+extern "C" lssm_status lssm_prefill(lssm_session* s, const uint32_t* tokens, uint32_t L, uint32_t* next_tokens) {
+    if (!s || !tokens) return fail(LSSM_ERR_INVALID_ARGUMENT, "lssm_prefill: null argument");
+    if (L == 0) return fail(LSSM_ERR_INVALID_ARGUMENT, "forward_prefill: L must be >= 1");
+    if (L > s->max_L) return fail(LSSM_ERR_INVALID_ARGUMENT, "forward_prefill: L exceeds workspace max_seq_len");
+    cudaSetDevice(s->ctx->device);
+    cudaStream_t st = s->ctx->stream;
+    const uint64_t nl0 = s->nl;
+    if (lssm_status r = forward_rows(s, tokens, L, st)) return r;
     if (lssm_status r = pick_tokens(s, s->lastrows, false, st)) return r;
     s->prefill_launches = s->nl - nl0;
     CU(cudaEventRecord(s->ev[1], st));
@@ -1199,6 +1299,119 @@ extern "C" lssm_status lssm_prefill(lssm_session* s, const uint32_t* tokens, uin
     cudaEventElapsedTime(&s->prefill_ms, s->ev[0], s->ev[1]);
     s->logits_valid = true;
     return check_err(s, "prefill");
+}
+
+// ---- scoring ---------------------------------------------------------------------
+// Device block of the scoring calls: logits of `run` rows, then targets and results of `rows` rows.
+struct ScoreBlock {
+    __half* logits;
+    uint32_t *targets, *ids;
+    float *logp, *entropy, *top;
+};
+static lssm_status score_block(lssm_session* s, size_t rows, size_t run, uint32_t top_k, ScoreBlock* b) {
+    const size_t lb = al256(run * s->V * 2), rb = al256(rows * 4), kb = al256(rows * top_k * 4), need = lb + 3 * rb + 2 * kb;
+    if (need > s->score_bytes) {
+        CU(cudaStreamSynchronize(s->ctx->stream));
+        if (s->d_score) cudaFree(s->d_score);
+        s->d_score = nullptr;
+        s->score_bytes = 0;
+        if (lssm_status r = s_alloc(reinterpret_cast<void**>(&s->d_score), need, "session: scoring")) return r;
+        s->score_bytes = need;
+    }
+    uint8_t* p = s->d_score;
+    b->logits = reinterpret_cast<__half*>(p); p += lb;
+    b->targets = reinterpret_cast<uint32_t*>(p); p += rb;
+    b->logp = reinterpret_cast<float*>(p); p += rb;
+    b->entropy = reinterpret_cast<float*>(p); p += rb;
+    b->ids = reinterpret_cast<uint32_t*>(p); p += kb;
+    b->top = reinterpret_cast<float*>(p);
+    return LSSM_OK;
+}
+static lssm_status score_checks(const lssm_session* s, const char* who, uint32_t top_k, const float* logp,
+                                const float* entropy, const uint32_t* ids, const float* top) {
+    if (s->comm) return fail(LSSM_ERR_STATE, "%s: the vocabulary of a tensor-parallel session is split over the ranks", who);
+    if (s->ctx->batch_active) return fail(LSSM_ERR_STATE, "%s: a batch is active", who);
+    if (top_k > LSSM_TOP_K_MAX || top_k > s->V)
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "%s: top_k must be at most %u and at most the vocabulary", who, LSSM_TOP_K_MAX);
+    if ((ids != nullptr) != (top_k > 0) || (top != nullptr) != (top_k > 0))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "%s: top_ids and top_logp are given exactly when top_k > 0", who);
+    if (!logp && !entropy && !top_k) return fail(LSSM_ERR_INVALID_ARGUMENT, "%s: no output given", who);
+    return LSSM_OK;
+}
+static lssm_status score_rows(lssm_session* s, const __half* logits, const ScoreBlock& b, size_t first, uint32_t n, uint32_t top_k,
+                              cudaStream_t st) {
+    LogprobsArgs a{};
+    a.logits = logits; a.targets = b.targets + first;
+    a.logp = b.logp + first; a.entropy = b.entropy + first;
+    if (top_k) { a.top_ids = b.ids + first * top_k; a.top_logp = b.top + first * top_k; }
+    a.rows = n; a.vocab = s->V; a.top_k = top_k; a.dtype = LSSM_DT_F16; a.row_stride = s->V;
+    a.sm_count = s->ctx->sm_count;
+    CU(launch_logprobs(a, st));
+    s->nl += 1;
+    return LSSM_OK;
+}
+static lssm_status score_results(const ScoreBlock& b, size_t rows, uint32_t top_k, float* logp, float* entropy, uint32_t* ids,
+                                 float* top, cudaStream_t st) {
+    if (logp) CU(cudaMemcpyAsync(logp, b.logp, rows * 4, cudaMemcpyDeviceToHost, st));
+    if (entropy) CU(cudaMemcpyAsync(entropy, b.entropy, rows * 4, cudaMemcpyDeviceToHost, st));
+    if (top_k) {
+        CU(cudaMemcpyAsync(ids, b.ids, rows * top_k * 4, cudaMemcpyDeviceToHost, st));
+        CU(cudaMemcpyAsync(top, b.top, rows * top_k * 4, cudaMemcpyDeviceToHost, st));
+    }
+    CU(cudaStreamSynchronize(st));
+    return LSSM_OK;
+}
+
+extern "C" lssm_status lssm_score(lssm_session* s, const uint32_t* tokens, uint32_t L, uint32_t top_k, float* logp,
+                                  float* entropy, uint32_t* top_ids, float* top_logp) {
+    if (!s || !tokens) return fail(LSSM_ERR_INVALID_ARGUMENT, "lssm_score: null argument");
+    if (L == 0) return fail(LSSM_ERR_INVALID_ARGUMENT, "lssm_score: L must be >= 1");
+    if (L > s->max_L) return fail(LSSM_ERR_INVALID_ARGUMENT, "lssm_score: L exceeds workspace max_seq_len");
+    if (lssm_status r = score_checks(s, "lssm_score", top_k, logp, entropy, top_ids, top_logp)) return r;
+    cudaSetDevice(s->ctx->device);
+    cudaStream_t st = s->ctx->stream;
+    const SsmHeader& h = s->m->img.hdr;
+    const size_t rows = (size_t)s->batch * L;
+    // the vocabulary's logits of a run of rows at a time: 64 MiB, at least a tile of the GEMM
+    const size_t run = std::min(rows, std::max<size_t>(128, ((size_t)64 << 20) / ((size_t)s->V * 2) / 128 * 128));
+    ScoreBlock b;
+    if (lssm_status r = score_block(s, rows, run, top_k, &b)) return r;
+    const uint64_t nl0 = s->nl;
+    if (lssm_status r = forward_rows(s, tokens, L, st)) return r;
+    // row i's target is token i + 1 of its sequence; the last row has none
+    CU(cudaMemsetAsync(b.targets, 0xFF, rows * 4, st));
+    if (L > 1)
+        CU(cudaMemcpy2DAsync(b.targets, (size_t)L * 4, s->d_tokens + 1, (size_t)L * 4, (size_t)(L - 1) * 4, s->batch,
+                             cudaMemcpyDeviceToDevice, st));
+    for (size_t r0 = 0; r0 < rows; r0 += run) {
+        const uint32_t n = (uint32_t)std::min(run, rows - r0);
+        if (lssm_status r = linear(s, s->lm_w, s->lm_dt, s->hidden + r0 * h.d_model, b.logits, n, s->V, h.d_model, s->norm_f, 0, st))
+            return r;
+        if (lssm_status r = score_rows(s, b.logits, b, r0, n, top_k, st)) return r;
+    }
+    if (lssm_status r = pick_tokens(s, s->lastrows, false, st)) return r;
+    s->prefill_launches = s->nl - nl0;
+    CU(cudaEventRecord(s->ev[1], st));
+    if (lssm_status r = score_results(b, rows, top_k, logp, entropy, top_ids, top_logp, st)) return r;
+    cudaEventElapsedTime(&s->prefill_ms, s->ev[0], s->ev[1]);
+    s->logits_valid = true;
+    return check_err(s, "score");
+}
+
+extern "C" lssm_status lssm_session_logprobs(lssm_session* s, const uint32_t* targets, uint32_t top_k, float* logp,
+                                             float* entropy, uint32_t* top_ids, float* top_logp) {
+    if (!s) return fail(LSSM_ERR_INVALID_ARGUMENT, "lssm_session_logprobs: null session");
+    if (lssm_status r = score_checks(s, "lssm_session_logprobs", top_k, logp, entropy, top_ids, top_logp)) return r;
+    if (logp && !targets) return fail(LSSM_ERR_INVALID_ARGUMENT, "lssm_session_logprobs: logp needs targets");
+    if (!s->logits_valid) return fail(LSSM_ERR_STATE, "lssm_session_logprobs: no logits computed yet");
+    cudaSetDevice(s->ctx->device);
+    cudaStream_t st = s->ctx->stream;
+    ScoreBlock b;
+    if (lssm_status r = score_block(s, s->batch, 0, top_k, &b)) return r;
+    if (targets) CU(cudaMemcpyAsync(b.targets, targets, (size_t)s->batch * 4, cudaMemcpyHostToDevice, st));
+    else CU(cudaMemsetAsync(b.targets, 0xFF, (size_t)s->batch * 4, st));
+    if (lssm_status r = score_rows(s, s->logits, b, 0, s->batch, top_k, st)) return r;
+    return score_results(b, s->batch, top_k, logp, entropy, top_ids, top_logp, st);
 }
 
 // One decode step on the device: input = s->hidden rows (already embedded), output:
@@ -1227,7 +1440,9 @@ extern "C" lssm_status lssm_decode(lssm_session* s, const uint32_t* first, uint3
     }
     CU(cudaMemcpyAsync(s->d_cur, first, (size_t)s->batch * 4, cudaMemcpyHostToDevice, st));
     CU(cudaMemsetAsync(s->d_step, 0, 4, st));
-    if (s->persist_ok && s->use_persist) {
+    const bool persistent = s->persist_ok && s->use_persist;
+    if (lssm_status r = states_to(s, s->state_bits && !persistent, st)) return r;
+    if (persistent) {
         // one cooperative launch runs all n_steps tokens (embedding gather included);
         // the kernel reads embedding rows directly, so the ids are range-checked here
         for (uint32_t b = 0; b < s->batch; ++b)

@@ -156,6 +156,8 @@ _SIGS = {
     "lssm_decode": [P, P, u32, P],
     "lssm_generate": [P, P, u32, u32, u32, P, C.POINTER(u32)],
     "lssm_session_logits": [P, P],
+    "lssm_score": [P, P, u32, u32, P, P, P, P],
+    "lssm_session_logprobs": [P, P, u32, P, P, P, P],
     "lssm_session_timing": [P, C.POINTER(f32), C.POINTER(f32)],
     "lssm_session_set_option": [P, C.c_char_p, C.c_int64],
     "lssm_session_launches": [P, C.POINTER(u64), C.POINTER(u64)],
@@ -647,6 +649,30 @@ class Session:
         out = np.zeros((self.batch, self.vocab), dtype=np.float32)
         check(lib().lssm_session_logits(self.h, out.ctypes.data_as(P)))
         return out
+
+    def score(self, tokens: np.ndarray, top_k: int = 0):
+        """Teacher-forced scoring of batch x L tokens (lssm_score): (logp, entropy), batch x L fp32, and
+        with top_k also (top_ids, top_logp), batch x L x top_k. logp[:, i] is the log probability of
+        tokens[:, i + 1] after tokens[:, : i + 1]; the last one is 0. The session continues as after prefill."""
+        t = np.ascontiguousarray(tokens, dtype=np.uint32).reshape(self.batch, -1)
+        return self._scored(t.shape, top_k, lambda *o: lib().lssm_score(
+            self.h, t.ctypes.data_as(P), t.shape[1], top_k, *o))
+
+    def logprobs(self, targets: np.ndarray, top_k: int = 0):
+        """Log probabilities of `targets` (one id per sequence) under the logits of the last position
+        computed, with entropy and alternatives (lssm_session_logprobs)."""
+        t = np.ascontiguousarray(targets, dtype=np.uint32).reshape(self.batch)
+        return self._scored(t.shape, top_k, lambda *o: lib().lssm_session_logprobs(
+            self.h, t.ctypes.data_as(P), top_k, *o))
+
+    @staticmethod
+    def _scored(shape, top_k, call):
+        out = [np.zeros(shape, np.float32), np.zeros(shape, np.float32)]
+        if top_k:
+            out += [np.zeros((*shape, top_k), np.uint32), np.zeros((*shape, top_k), np.float32)]
+        ptrs = [a.ctypes.data_as(P) for a in out] + [None] * (4 - len(out))
+        check(call(*ptrs))
+        return tuple(out)
 
     def timing(self):
         a, b = f32(), f32()
