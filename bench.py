@@ -668,6 +668,9 @@ def run_batched(args, world, rank, local, dist, ctx=None, model=None, steps=None
     if own:
         model = lssm.Model.synthesize(ctx, lssm.hparams(**HP27), seed=0, int4=True)
     sess = lssm.Session(ctx, model, batch=per, max_seq_len=plen)
+    if args.state_bits and own:   # the default run's embedded workload keeps fp32 states
+        sess.set_option("state_bits", args.state_bits)
+        sess.set_option("persistent", 0)
     rng = np.random.default_rng(2000 + rank)
     prompts = rng.integers(0, VOCAB_IDS, size=(per, plen)).astype(np.uint32)
 
@@ -708,7 +711,10 @@ def run_batched(args, world, rank, local, dist, ctx=None, model=None, steps=None
     (e_max,) = allreduce_max(dist, [e_s], local)
     assert out.shape == (per, steps_new + 1)
     bpt = decode_bytes_per_token(HP27)
-    state_b = HP27["n_layer"] * (bpt["per_layer"]["ssd_state_rw"] + bpt["per_layer"]["conv_state_rw"])
+    ssd_b = bpt["per_layer"]["ssd_state_rw"]
+    if args.state_bits and own:   # codes read every step and written once in 16, half a window of tokens read
+        ssd_b = ssd_b / 8 * (args.state_bits / 8) * (1 + 1 / 16) + 8.5 * 80 * 64 * 2
+    state_b = HP27["n_layer"] * (ssd_b + bpt["per_layer"]["conv_state_rw"])
     step_bytes = (bpt["total"] - HP27["n_layer"] * (bpt["per_layer"]["ssd_state_rw"] + bpt["per_layer"]["conv_state_rw"])
                   + per * state_b)   # weights once per step per GPU + every sequence's state R+W
     ms_step = tot_dec / n_steps / steps_new
@@ -717,7 +723,8 @@ def run_batched(args, world, rank, local, dist, ctx=None, model=None, steps=None
         line = {
             "metric": METRIC, "value": decode_tok_s, "unit": "tok/s", "n_gpus": world, "steps": n_steps,
             "warmup": n_warm, "ms_per_step": (tot_pre + tot_dec) / n_steps, "higher_is_better": True,
-            "scaling": "strong", "vs_baseline": None, "dtype": "f16 activations, int4_b32 weights, f32 accum",
+            "scaling": "strong", "vs_baseline": None, "dtype": "f16 activations, int4_b32 weights, f32 accum"
+                     + (f", int{args.state_bits} decode states" if args.state_bits and own else ""),
             "data": "synthetic (seeded random-init weights in the reference .ssm INT4_B32 layout, random prompt ids)",
             "config": {"workload": f"batched decode: {total} sequences x ({plen} prompt + {steps_new} greedy steps)",
                        "model": "mamba2-2.7b-shape (64L, d_model 2560, 80x64 heads, d_state 128, vocab 50288)",
@@ -848,6 +855,8 @@ def main():
     ap.add_argument("--tp-prompt", type=int, default=4096)
     ap.add_argument("--tp-new", type=int, default=128)
     ap.add_argument("--seqs", type=int, default=64)
+    ap.add_argument("--state-bits", type=int, default=0, choices=[0, 8, 16],
+                    help="--workload batched: decode over a quantised state cache (0: fp32 states)")
     ap.add_argument("--batched-prompt", type=int, default=512)
     ap.add_argument("--batched-new", type=int, default=256)
     ap.add_argument("--kernel", default=None,

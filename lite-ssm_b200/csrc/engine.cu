@@ -1019,20 +1019,27 @@ static StateCacheArgs cache_args(const lssm_session* s, uint32_t layer) {
     a.dt_min = 1e-6f; a.dt_max = 1e6f; a.has_D = 1;
     return a;
 }
-// The states to where the next call wants them: the cache (per-op decode under "state_bits") or fp32.
-static lssm_status states_to(lssm_session* s, bool cache, cudaStream_t st) {
-    if (s->in_cache == cache) return LSSM_OK;
+// The states from where they are to the other place: into the cache (`in_cache` is set by the caller, before it
+// captures a step over it) or back to fp32.
+static lssm_status states_to_cache(lssm_session* s, cudaStream_t st) {
     for (uint32_t l = 0; l < s->m->img.hdr.n_layer; ++l) {
-        const StateCacheArgs a = cache_args(s, l);
-        CU(cache ? launch_state_store(a, st) : launch_state_load(a, st));
+        CU(launch_state_store(cache_args(s, l), st));
         s->nl += 1;
     }
-    s->in_cache = cache;
+    return LSSM_OK;
+}
+static lssm_status states_to_f32(lssm_session* s, cudaStream_t st) {
+    if (!s->in_cache) return LSSM_OK;
+    for (uint32_t l = 0; l < s->m->img.hdr.n_layer; ++l) {
+        CU(launch_state_load(cache_args(s, l), st));
+        s->nl += 1;
+    }
+    s->in_cache = false;
     return LSSM_OK;
 }
 static lssm_status set_state_cache(lssm_session* s, uint32_t bits, uint32_t window) {
     if (bits == s->state_bits && window == s->state_window) return LSSM_OK;
-    if (lssm_status r = states_to(s, false, s->ctx->stream)) return r;
+    if (lssm_status r = states_to_f32(s, s->ctx->stream)) return r;
     CU(cudaStreamSynchronize(s->ctx->stream));
     if (s->graph) { cudaGraphExecDestroy(s->graph); s->graph = nullptr; }
     if (s->d_cache) { cudaFree(s->d_cache); s->d_cache = nullptr; }
@@ -1270,7 +1277,7 @@ static lssm_status forward_rows(lssm_session* s, const uint32_t* tokens, uint32_
     lssm_model* m = s->m;
     const SsmHeader& h = m->img.hdr;
     const uint32_t rows = s->batch * L;
-    if (lssm_status r = states_to(s, false, st)) return r;
+    if (lssm_status r = states_to_f32(s, st)) return r;
     CU(cudaMemcpyAsync(s->d_tokens, tokens, (size_t)rows * 4, cudaMemcpyHostToDevice, st));
     CU(cudaEventRecord(s->ev[0], st));   // device timing starts with the tokens resident in HBM
     CU(launch_embed_gather(s->d_tokens, W(m, m->embed), s->hidden, rows, h.d_model, h.vocab_size, s->d_err, st));
@@ -1441,8 +1448,8 @@ extern "C" lssm_status lssm_decode(lssm_session* s, const uint32_t* first, uint3
     CU(cudaMemcpyAsync(s->d_cur, first, (size_t)s->batch * 4, cudaMemcpyHostToDevice, st));
     CU(cudaMemsetAsync(s->d_step, 0, 4, st));
     const bool persistent = s->persist_ok && s->use_persist;
-    if (lssm_status r = states_to(s, s->state_bits && !persistent, st)) return r;
     if (persistent) {
+        if (lssm_status r = states_to_f32(s, st)) return r;
         // one cooperative launch runs all n_steps tokens (embedding gather included);
         // the kernel reads embedding rows directly, so the ids are range-checked here
         for (uint32_t b = 0; b < s->batch; ++b)
@@ -1472,6 +1479,8 @@ extern "C" lssm_status lssm_decode(lssm_session* s, const uint32_t* first, uint3
         return check_err(s, "decode");
     }
     CU(launch_embed_gather(s->d_cur, W(m, m->embed), s->hidden, s->batch, h.d_model, h.vocab_size, s->d_err, st));
+    const bool quantise = s->state_bits && !s->in_cache;
+    s->in_cache = s->state_bits != 0;
     if (s->use_graph && !s->graph) {
         cudaGraph_t g;
         CU(cudaStreamBeginCapture(st, cudaStreamCaptureModeThreadLocal));
@@ -1479,13 +1488,20 @@ extern "C" lssm_status lssm_decode(lssm_session* s, const uint32_t* first, uint3
         lssm_status r = decode_step_body(s, st);
         s->decode_step_launches = s->nl - nl0;
         cudaError_t e = cudaStreamEndCapture(st, &g);
+        if (r || e != cudaSuccess) s->in_cache = s->in_cache && !quantise;
         if (r) { if (e == cudaSuccess) cudaGraphDestroy(g); return r; }
         if (e != cudaSuccess) return cuda_fail(e, "decode graph capture");
         e = cudaGraphInstantiate(&s->graph, g, 0);
         cudaGraphDestroy(g);
-        if (e != cudaSuccess) { s->graph = nullptr; return cuda_fail(e, "decode graph instantiate"); }
+        if (e != cudaSuccess) {
+            s->graph = nullptr;
+            s->in_cache = s->in_cache && !quantise;
+            return cuda_fail(e, "decode graph instantiate");
+        }
     }
     CU(cudaEventRecord(s->ev[2], st));
+    if (quantise)
+        if (lssm_status r = states_to_cache(s, st)) { s->in_cache = false; return r; }
     for (uint32_t i = 0; i < n_steps; ++i) {
         if (s->graph) CU(cudaGraphLaunch(s->graph, st));
         else {
