@@ -41,14 +41,15 @@ struct RowQuant {
         inv = scale > 0.0f ? __frcp_rn(scale) : 0.0f;
         half = scale > 0.0f ? 0.5f * scale : INFINITY;
     }
+    // of a scale that is worked out already
+    struct Known { float scale, inv; };
+    __device__ __forceinline__ RowQuant(Known k) : scale(k.scale), inv(k.inv) {
+        half = scale > 0.0f ? 0.5f * scale : INFINITY;
+        sound = scale == scale;
+    }
     // what lane l of the warp has
     __device__ __forceinline__ RowQuant of_lane(int l) const {
-        RowQuant z = *this;
-        z.scale = __shfl_sync(0xffffffffu, scale, l);
-        z.inv = __shfl_sync(0xffffffffu, inv, l);
-        z.half = z.scale > 0.0f ? 0.5f * z.scale : INFINITY;
-        z.sound = z.scale == z.scale;
-        return z;
+        return RowQuant(Known{__shfl_sync(0xffffffffu, scale, l), __shfl_sync(0xffffffffu, inv, l)});
     }
 };
 // Codes of four elements as whole numbers in the low bits of the results. Added to 1.5 * 2^23, v / scale is rounded
@@ -120,94 +121,156 @@ __device__ __forceinline__ void window_weights(float a, float dt, uint32_t lane,
 
 constexpr int SC_THREADS = 256;
 
-// General shapes: one CTA per (sequence, head), a warp per row of N.
-// MODE 0: step (y, window append, requantise when full); MODE 1: load (the state as it stands).
-template <typename Code, int MODE>
-__global__ void __launch_bounds__(SC_THREADS) k_state_cached(StateCacheArgs a) {
-    __shared__ float w[LSSM_STATE_WINDOW_MAX];
-    __shared__ float s_alpha;
-    const uint32_t h = blockIdx.x % a.H, b = blockIdx.x / a.H, g = h / (a.H / a.G);
-    const uint32_t lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-    const uint64_t bh = (uint64_t)b * a.H + h;
+// Any shape: one CTA per (sequence, head), ANY_ROWS rows at a time; lane l of a warp takes elements l, l + 32, ... of a
+// row, so neighbours are read and written together whatever N and the arrays' alignment are.
+// A step: S_q C of the rows by warps, C . B_j of the window's tokens by warps, then y by a thread a row.
+// A fold or a load: a warp keeps 32 elements of every B_j in registers (KB * 16 of them) and walks down the rows.
+constexpr uint32_t ANY_ROWS = 128;
+template <typename Code, int MODE, int KB>
+__global__ void __launch_bounds__(SC_THREADS) k_state_any(StateCacheArgs a) {
     constexpr float Q = sizeof(Code) == 1 ? 127.0f : 32767.0f;
-    uint32_t n = a.fill[bh];
-    if (MODE == 0) n = n < a.W ? n : a.W - 1;
-    const uint32_t count = MODE == 0 ? n + 1 : (n < a.W ? n : a.W);
-    if (wid == 0) {
-        const float rate = -expf(__half2float(a.A_log[h]));
-        float dt = 0.0f;
-        if (lane < count) dt = a.win_dt[bh * a.W + lane];
-        if (MODE == 0 && lane == n)
-            dt = token_dt(__half2float(a.dt_raw[b * a.dt_bs + h]) + __half2float(a.dt_bias[h]), a.dt_min, a.dt_max);
-        float wj, al;
-        window_weights(rate, dt, lane, count, &wj, &al);
-        w[lane] = wj;
-        if (lane == 0) s_alpha = al;
-        if (MODE == 0 && lane == n) a.win_dt[bh * a.W + n] = dt;
-    }
-    __syncthreads();
-    const float alpha = s_alpha;
-    const uint64_t xrow = (uint64_t)a.H * a.P, brow = (uint64_t)a.G * a.N;
+    constexpr int WARPS = SC_THREADS / 32, J = 16 * KB;
+    __shared__ __align__(16) float s_xw[ANY_ROWS][J + 4];   // w_j x_j[p], 0 behind the window's tokens
+    __shared__ float s_w[32], s_cb[32], s_row[ANY_ROWS], s_scale[ANY_ROWS], s_inv[ANY_ROWS], s_alpha;
+    __shared__ uint32_t s_top[ANY_ROWS];
+    const uint32_t h = blockIdx.x % a.H, b = blockIdx.x / a.H, g = h / (a.H / a.G);
+    const uint32_t tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+    const uint64_t bh = blockIdx.x, xrow = (uint64_t)a.H * a.P, brow = (uint64_t)a.G * a.N;
+    // a step's token is number n of the window; `count` tokens with it
+    const uint32_t filled = a.fill[bh], n = MODE == 0 ? min(filled, a.W - 1) : a.W;
+    const uint32_t count = MODE == 0 ? n + 1 : min(filled, a.W);
+    const bool fold = MODE == 0 && count == a.W;
     const __half* wx = a.win_x + (uint64_t)b * a.W * xrow + (uint64_t)h * a.P;
-    const __half* wB = a.win_B + (uint64_t)b * a.W * brow + (uint64_t)g * a.N;
+    __half* wB = a.win_B + (uint64_t)b * a.W * brow + (uint64_t)g * a.N;
     const __half* xn = MODE == 0 ? a.x + b * a.x_bs + (uint64_t)h * a.P : nullptr;
     const __half* Bn = MODE == 0 ? a.B + b * a.bc_bs + (uint64_t)g * a.N : nullptr;
     const __half* Cn = MODE == 0 ? a.C + b * a.bc_bs + (uint64_t)g * a.N : nullptr;
-    const bool fold = MODE == 0 && n + 1 == a.W;
-    for (uint32_t p = wid; p < a.P; p += SC_THREADS / 32) {
-        Code* row = static_cast<Code*>(a.codes) + (bh * a.P + p) * a.N;
-        const float as = alpha * a.scales[bh * a.P + p];
-        // x of every window token of this row, scaled: lane j holds token j
-        float xw = 0.0f;
-        if (lane < count) xw = w[lane] * __half2float(MODE == 0 && lane == n ? xn[p] : wx[lane * xrow + p]);
-        auto state = [&](uint32_t i, bool in) {
-            float v = in ? as * (float)row[i] : 0.0f;
-            for (uint32_t j = 0; j < count; ++j) {
-                const float xj = __shfl_sync(0xffffffffu, xw, j);
-                if (in) v = fmaf(xj, __half2float(MODE == 0 && j == n ? Bn[i] : wB[j * brow + i]), v);
-            }
-            return v;
-        };
-        float acc = 0.0f, amax = 0.0f;
-        for (uint32_t i0 = 0; i0 < a.N; i0 += 32) {
-            const uint32_t i = i0 + lane;
-            const bool in = i < a.N;
-            const float v = state(i, in);
-            if (MODE == 1) {
-                if (in) store_any(a.state, (bh * a.P + p) * a.N + i, a.state_dtype, v);
-            } else if (in) {
-                acc = fmaf(v, __half2float(Cn[i]), acc);
-                amax = max_nan(amax, fabsf(v));
-            }
+    auto token_x = [&](uint32_t j) { return MODE == 0 && j == n ? xn : wx + j * xrow; };
+    auto token_B = [&](uint32_t j) { return MODE == 0 && j == n ? Bn : wB + j * brow; };
+    if (wid == 0) {
+        float dt = 0.0f;
+        if (lane < count && lane != n) dt = a.win_dt[bh * a.W + lane];
+        if (MODE == 0 && lane == n)
+            dt = token_dt(__half2float(a.dt_raw[b * a.dt_bs + h]) + __half2float(a.dt_bias[h]), a.dt_min, a.dt_max);
+        float wj, al;
+        window_weights(-expf(__half2float(a.A_log[h])), dt, lane, count, &wj, &al);
+        s_w[lane] = wj;
+        if (lane == 0) s_alpha = al;
+        if (MODE == 0 && lane == n) a.win_dt[bh * a.W + n] = dt;
+    }
+    if (MODE == 0)
+        for (uint32_t j = wid; j < count; j += WARPS) {
+            const __half* B = token_B(j);
+            float d = 0.0f;
+            for (uint32_t i = lane; i < a.N; i += 32) d = fmaf(__half2float(B[i]), __half2float(Cn[i]), d);
+            d = warp_sum(d);
+            if (lane == 0) s_cb[j] = d;
         }
+    __syncthreads();
+    const float alpha = s_alpha;
+    const uint32_t chunks = (a.N + 31) / 32, splits = chunks >= WARPS ? 1 : WARPS / chunks;
+    for (uint32_t p0 = 0; p0 < a.P; p0 += ANY_ROWS) {
+        const uint32_t rows = min(ANY_ROWS, a.P - p0);
+        Code* codes = static_cast<Code*>(a.codes) + (bh * a.P + p0) * a.N;
+        float* scales = a.scales + bh * a.P + p0;
         if (MODE == 0) {
-            acc = warp_sum(acc);
-            if (lane == 0) {
-                const float xv = __half2float(xn[p]);
-                const float Dh = a.has_D ? __half2float(a.D[h]) : 0.0f;
-                const __half yh = __float2half_rn(acc + Dh * xv);
-                const uint64_t o = (uint64_t)h * a.P + p;
-                a.y[b * a.y_bs + o] =
-                    a.z ? __float2half_rn(silu(__half2float(a.z[b * a.z_bs + o])) * __half2float(yh)) : yh;
-                a.win_x[((uint64_t)b * a.W + n) * xrow + o] = xn[p];
-            }
-            if (fold) {
-                const RowQuant z(warp_max_nan(amax), Q);
-                for (uint32_t i0 = 0; i0 < a.N; i0 += 32) {
-                    const uint32_t i = i0 + lane;
-                    const float v = state(i, i < a.N);
-                    if (i < a.N) row[i] = quantise1<Code>(v, z);
+            for (uint32_t p = wid * 4; p < rows; p += WARPS * 4) {
+                float d[4] = {};
+                for (uint32_t i = lane; i < a.N; i += 32) {
+                    const float c = __half2float(Cn[i]);
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; ++r)
+                        if (p + r < rows) d[r] = fmaf((float)codes[(uint64_t)(p + r) * a.N + i], c, d[r]);
                 }
-                if (lane == 0) a.scales[bh * a.P + p] = z.scale;
+#pragma unroll
+                for (uint32_t r = 0; r < 4; ++r) {
+                    d[r] = warp_sum(d[r]);
+                    if (lane == r && p + r < rows) s_row[p + r] = d[r];
+                }
             }
+            __syncthreads();
+            if (tid < rows) {
+                const uint64_t o = (uint64_t)h * a.P + p0 + tid;
+                float yw = 0.0f;
+                for (uint32_t j = 0; j < count; ++j) yw = fmaf(s_w[j] * s_cb[j], __half2float(token_x(j)[p0 + tid]), yw);
+                const __half xh = xn[p0 + tid];
+                const float Dh = a.has_D ? __half2float(a.D[h]) : 0.0f;
+                const __half yh = __float2half_rn(fmaf(alpha * scales[tid], s_row[tid], yw) + Dh * __half2float(xh));
+                a.y[b * a.y_bs + o] = a.z ? __float2half_rn(silu(__half2float(a.z[b * a.z_bs + o])) * __half2float(yh)) : yh;
+                a.win_x[((uint64_t)b * a.W + n) * xrow + o] = xh;
+            }
+            __syncthreads();
+            if (!fold) continue;
+        }
+        for (uint32_t i = tid; i < rows * J; i += SC_THREADS) {
+            const uint32_t p = i % rows, j = i / rows;
+            s_xw[p][j] = j < count ? s_w[j] * __half2float(token_x(j)[p0 + p]) : 0.0f;
+        }
+        if (tid < rows) {
+            s_row[tid] = alpha * scales[tid];
+            s_top[tid] = 0;
+        }
+        __syncthreads();
+        // PASS 0: the rows' largest magnitudes (fold) or the state itself (load); 1: the codes. A walk down the rows
+        // for every 32 elements.
+        auto walk = [&](auto pass) {
+            for (uint32_t task = wid; task < chunks * splits; task += WARPS) {
+                const uint32_t i = task % chunks * 32 + lane;
+                const bool in = i < a.N;
+                float B[J];
+#pragma unroll
+                for (uint32_t j = 0; j < J; ++j) B[j] = in && j < count ? __half2float(token_B(j)[i]) : 0.0f;
+                for (uint32_t p = task / chunks * 2; p < rows; p += splits * 2) {
+                    float v[2];
+#pragma unroll
+                    for (uint32_t r = 0; r < 2; ++r) v[r] = in && p + r < rows ? s_row[p + r] * (float)codes[(uint64_t)(p + r) * a.N + i] : 0.0f;
+#pragma unroll
+                    for (uint32_t j = 0; j < J; j += 4) {
+                        if (j >= count) break;
+#pragma unroll
+                        for (uint32_t r = 0; r < 2; ++r) {
+                            const float4 x = *reinterpret_cast<const float4*>(&s_xw[min(p + r, rows - 1)][j]);
+                            v[r] = fmaf(x.x, B[j], v[r]);
+                            v[r] = fmaf(x.y, B[j + 1], v[r]);
+                            v[r] = fmaf(x.z, B[j + 2], v[r]);
+                            v[r] = fmaf(x.w, B[j + 3], v[r]);
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t r = 0; r < 2; ++r) {
+                        if (p + r >= rows) break;
+                        const uint64_t at = (uint64_t)(p + r) * a.N + i;
+                        if constexpr (MODE == 1) {
+                            if (in) store_any(a.state, (bh * a.P + p0) * a.N + at, a.state_dtype, v[r]);
+                        } else if constexpr (decltype(pass)::value == 0) {
+                            // the bits of |v| order as the values do, NaN above infinity
+                            const uint32_t top = __reduce_max_sync(0xffffffffu, in ? __float_as_uint(v[r]) & 0x7FFFFFFFu : 0u);
+                            if (lane == 0) atomicMax(&s_top[p + r], top);
+                        } else if (in) {
+                            codes[at] = quantise1<Code>(v[r], RowQuant(RowQuant::Known{s_scale[p + r], s_inv[p + r]}));
+                        }
+                    }
+                }
+            }
+        };
+        walk(std::integral_constant<int, 0>());
+        __syncthreads();
+        if (MODE == 0) {
+            if (tid < rows) {
+                const RowQuant z(__uint_as_float(s_top[tid]), Q);
+                scales[tid] = s_scale[tid] = z.scale;
+                s_inv[tid] = z.inv;
+            }
+            __syncthreads();
+            walk(std::integral_constant<int, 1>());
+            __syncthreads();
         }
     }
     if (MODE == 0) {
         // the first head of a group keeps the group's B row; every head takes row n from its argument
         if (h % (a.H / a.G) == 0)
-            for (uint32_t i = threadIdx.x; i < a.N; i += SC_THREADS)
-                a.win_B[((uint64_t)b * a.W + n) * brow + (uint64_t)g * a.N + i] = Bn[i];
-        if (threadIdx.x == 0) a.fill[bh] = fold ? 0 : n + 1;
+            for (uint32_t i = tid; i < a.N; i += SC_THREADS) wB[n * brow + i] = Bn[i];
+        if (tid == 0) a.fill[bh] = fold ? 0 : count;
     }
 }
 
@@ -633,7 +696,8 @@ cudaError_t launch_cached(const StateCacheArgs& a, cudaStream_t s) {
     if (MODE == 0) tc = tc && aligned(a.x, 16) && aligned(a.B, 16) && aligned(a.C, 16) && a.bc_bs % 8 == 0 && a.x_bs % 8 == 0;
     else tc = tc && aligned(a.state, 16);
     if (!tc) {
-        k_state_cached<Code, MODE><<<a.batch * a.H, SC_THREADS, 0, s>>>(a);
+        if (a.W <= 16) k_state_any<Code, MODE, 1><<<a.batch * a.H, SC_THREADS, 0, s>>>(a);
+        else k_state_any<Code, MODE, 2><<<a.batch * a.H, SC_THREADS, 0, s>>>(a);
         return cudaGetLastError();
     }
     // Heads of a group share the window's B and what is computed from it: as many as 32 KB of codes allow, fewer
