@@ -296,14 +296,19 @@ __device__ __forceinline__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t
     constexpr int VEC = 16 / sizeof(T);
     const uint32_t tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const uint32_t bound = sh.bound;
-    const bool chosen = tkey >= bound;
-    const uint32_t votes = __ballot_sync(FULL, chosen);
-    uint32_t at = 0;
-    if (lane == 0 && votes) at = atomicAdd(&sh.nsel, __popc(votes));
-    at = __shfl_sync(FULL, at, 0) + __popc(votes & ((1u << lane) - 1));
-    if (chosen) sh.sel[at] = (uint8_t)(dealt ? lane * LP_WARPS + wid : tid);
-    __syncthreads();
-    const uint32_t nsel = sh.nsel;
+    uint32_t nsel = 0;
+    // the threads that may hold an entry at or above the bound (ties), or one above it
+    auto choose = [&](bool ties) {
+        const bool chosen = ties ? tkey >= bound : tkey > bound;
+        const uint32_t votes = __ballot_sync(FULL, chosen);
+        uint32_t at = 0;
+        if (lane == 0 && votes) at = atomicAdd(&sh.nsel, __popc(votes));
+        at = __shfl_sync(FULL, at, 0) + __popc(votes & ((1u << lane) - 1));
+        if (chosen) sh.sel[at] = (uint8_t)(dealt ? lane * LP_WARPS + wid : tid);
+        __syncthreads();
+        nsel = sh.nsel;
+    };
+    choose(true);
     const float bv = key_value(bound);
     const bool level = nsel > LP_THREADS / 4;   // many threads reach the bound: a masked or constant row
     auto collect = [&](bool ties) {
@@ -353,8 +358,9 @@ __device__ __forceinline__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t
         // Many equal to the bound: those above it first, then of the equal ones as many as are missing,
         // in the order of their index.
         __syncthreads();
-        if (tid == 0) { sh.count = 0; sh.nhits = 0; }
+        if (tid == 0) { sh.count = 0; sh.nhits = 0; sh.nsel = 0; }
         __syncthreads();
+        choose(false);
         collect(false);
         n = sh.count;
         if (sh.nhits <= LP_HITS && n <= LP_CAND) {

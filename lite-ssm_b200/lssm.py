@@ -349,6 +349,8 @@ class DeviceView:
     """Device memory that the caller owns (a torch tensor's data_ptr(), a part of a
     DeviceBuffer), for calls that take a buffer. The caller keeps it alive."""
 
+    __slots__ = ("ctx", "ptr")
+
     def __init__(self, ctx: Ctx, ptr: int):
         self.ctx = ctx
         self.ptr = P(ptr)
