@@ -293,6 +293,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the same from zero
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                               uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { uint32_t u; memcpy(&u, &h, 4); return u; }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { __half2 h; memcpy(&h, &u, 4); return h; }
 // Two unsigned bytes of w (chosen by sel, the 0x64 bytes from the constant) as f16 minus `off`: exact, 1024 + byte is.
@@ -400,12 +407,6 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
     uint8_t* codes = static_cast<uint8_t*>(a.codes) + (uint64_t)bh0 * a.P * Sh::ROW;
     float* scales = a.scales + (uint64_t)bh0 * a.P;
     const uint32_t filled = a.fill[bh0];
-    {
-        const uint8_t* from = codes + tid * 16;
-        constexpr uint32_t STEP = TC_THREADS / Sh::PIECES;   // rows a round, a multiple of 8: the exchange repeats
-        uint32_t to = sm0 + Sh::piece(tid / Sh::PIECES, tid % Sh::PIECES);
-        for (uint32_t r = tid / Sh::PIECES; r < rows; r += STEP, from += TC_THREADS * 16, to += TC_THREADS * 16) copy_async16(to, from);
-    }
     // what warp w < nh needs for head w's weights, and this thread's row
     float p_dt = 0.0f;
     __half p_raw = __ushort_as_half(0), p_bias = p_raw, p_A = p_raw, p_D = p_raw;
@@ -420,6 +421,12 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
         }
     }
     const float my_scale = tid < rows ? scales[tid] : 0.0f;
+    {
+        const uint8_t* from = codes + tid * 16;
+        constexpr uint32_t STEP = TC_THREADS / Sh::PIECES;   // rows a round, a multiple of 8: the exchange repeats
+        uint32_t to = sm0 + Sh::piece(tid / Sh::PIECES, tid % Sh::PIECES);
+        for (uint32_t r = tid / Sh::PIECES; r < rows; r += STEP, from += TC_THREADS * 16, to += TC_THREADS * 16) copy_async16(to, from);
+    }
     // A step's token is number n of the window; `count` tokens with it. All heads of a sequence have the same.
     const uint32_t n = MODE == 0 ? min(filled, a.W - 1) : a.W, count = MODE == 0 ? n + 1 : min(filled, a.W);
     const bool fold = MODE == 0 && count == a.W;
@@ -465,7 +472,10 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
             const uint32_t jp = i / (TC_N / 2), e = i % (TC_N / 2) * 2;
             const uint8_t* from = sm + sh.B + 2 * jp * Sh::B_PITCH + e * 2;
             const uint32_t p0 = *reinterpret_cast<const uint32_t*>(from), p1 = *reinterpret_cast<const uint32_t*>(from + Sh::B_PITCH);
-            *reinterpret_cast<uint2*>(&pairs[jp][e]) = make_uint2(__byte_perm(p0, p1, 0x5410), __byte_perm(p0, p1, 0x7632));
+            // of every four elements in the order 0, 2, 1, 3: a lane uses 0 and 2, or 1 and 3, of them
+            const uint32_t at = (e & ~3u) + (e >> 1 & 1);
+            pairs[jp][at] = __byte_perm(p0, p1, 0x5410);
+            pairs[jp][at + 2] = __byte_perm(p0, p1, 0x7632);
         }
         if (MODE == 1) __syncthreads();
     }
@@ -562,7 +572,6 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
     const uint32_t ldm = sm0 + sh.x + ((lane & 7) + (lane >> 4 & 1) * 8) * sh.x_pitch + (lane >> 3 & 1) * 16;
     for (uint32_t tile = wid; tile < rows / 16; tile += TC_WARPS) {
         const uint32_t row = tile * 16 + g, hh = head_of(tile * 16), sw = Sh::swap(row);   // of row + 8, too
-        const uint8_t* r0 = sm + row * Sh::ROW;
         const float as[2] = {s_as[row], s_as[row + 8]};
         // w_j x_j[p] of the lane's tokens: [0], [1] row g, tokens 2t, 2t + 1; [2], [3] row g + 8; [4] .. [7] tokens + 8
         float xw[KB * 8];
@@ -584,35 +593,39 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
         for (int k = 0; k < KB; ++k)
 #pragma unroll
             for (int i = 0; i < 4; ++i) split2(xw[8 * k + 2 * i] * p2.up, xw[8 * k + 2 * i + 1] * p2.up, &ah[k][i], &al[k][i]);
-        // elements 16 q + 4 t .. + 3 of the state, rows g and g + 8
-        auto word_at = [&](int q) {
-            const uint32_t byte = (16 * q + 4 * t) * sizeof(Code);
-            return (((byte >> 4) ^ sw) << 4) + (byte & 15);
-        };
-        const uint32_t pair0 = 4 * (g >> 1) + (g & 1);
+        // elements 16 q + 4 t .. + 3 of the state, rows g and g + 8. Their codes: piece q (8 bits; 16 bits: 2 q + t / 2),
+        // exchanged, so the address for q differs from the one for 0 in the bits of q alone
+        const uint32_t in_piece = 4 * t * sizeof(Code), at0 = row * Sh::ROW + (((in_piece >> 4) ^ sw) << 4) + (in_piece & 15);
+        auto word_at = [&](int q) { return at0 ^ (uint32_t)(q * 16 * sizeof(Code)); };
+        const uint32_t* pair0 = &pairs[t][4 * (g >> 1) + 2 * (g & 1)];
         auto word = [&](int q, float (&s)[2][4]) {
             float cu[4], cv[4];
-            const uint32_t at = word_at(q);
-            code_values<Code>(r0 + at, cu);
-            code_values<Code>(r0 + 8 * Sh::ROW + at, cv);
+            const uint8_t* at = sm + word_at(q);
+            code_values<Code>(at, cu);
+            code_values<Code>(at + 8 * Sh::ROW, cv);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                // column c of the product is element 16 q + 4 (c / 2) + c % 2 + 2 half: a lane gets what its codes are
-                float d[4] = {};
-                const int e = 16 * q + pair0 + 2 * half;
-                if (MODE == 0 || count) {
+            for (int i = 0; i < 4; ++i) { s[0][i] = as[0] * cu[i]; s[1][i] = as[1] * cv[i]; }
+            if (MODE == 1 && !count) return;
+            // column c of a product is element 16 q + 4 (c / 2) + c % 2 + 2 half: a lane gets what its codes are
+            float d[2][4];
 #pragma unroll
-                    for (int k = 0; k < KB; ++k) {
-                        const uint32_t b0 = pairs[8 * k + t][e], b1 = pairs[8 * k + t + 4][e];
-                        mma16816(d, ah[k][0], ah[k][1], ah[k][2], ah[k][3], b0, b1);
-                        mma16816(d, al[k][0], al[k][1], al[k][2], al[k][3], b0, b1);
-                    }
+            for (int k = 0; k < KB; ++k) {
+                const uint2 b0 = *reinterpret_cast<const uint2*>(pair0 + 8 * k * Sh::PAIR_PITCH + 16 * q);
+                const uint2 b1 = *reinterpret_cast<const uint2*>(pair0 + (8 * k + 4) * Sh::PAIR_PITCH + 16 * q);
+                if (k == 0) {
+                    mma16816_first(d[0], ah[k][0], ah[k][1], ah[k][2], ah[k][3], b0.x, b1.x);
+                    mma16816_first(d[1], ah[k][0], ah[k][1], ah[k][2], ah[k][3], b0.y, b1.y);
+                } else {
+                    mma16816(d[0], ah[k][0], ah[k][1], ah[k][2], ah[k][3], b0.x, b1.x);
+                    mma16816(d[1], ah[k][0], ah[k][1], ah[k][2], ah[k][3], b0.y, b1.y);
                 }
+                mma16816(d[0], al[k][0], al[k][1], al[k][2], al[k][3], b0.x, b1.x);
+                mma16816(d[1], al[k][0], al[k][1], al[k][2], al[k][3], b0.y, b1.y);
+            }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    s[0][2 * half + i] = fmaf(d[i], p2.down, as[0] * cu[2 * half + i]);
-                    s[1][2 * half + i] = fmaf(d[2 + i], p2.down, as[1] * cv[2 * half + i]);
-                }
+            for (int i = 0; i < 4; ++i) {
+                s[0][i] = fmaf(d[i >> 1][i & 1], p2.down, s[0][i]);
+                s[1][i] = fmaf(d[i >> 1][2 + (i & 1)], p2.down, s[1][i]);
             }
         };
         if constexpr (MODE == 1) {
@@ -655,14 +668,13 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
 #pragma unroll
                 for (int r = 0; r < 2; ++r) amax[r] = max_keep_nan(amax[r], __shfl_xor_sync(0xffffffffu, amax[r], o));
             const RowQuant z0(amax[0], Q), z1(amax[1], Q);
-            uint8_t* w0 = sm + row * Sh::ROW;
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
                 float s[2][4];
                 word(q, s);
-                const uint32_t at = word_at(q);
-                store_codes4(reinterpret_cast<Code*>(w0 + at), s[0], z0);
-                store_codes4(reinterpret_cast<Code*>(w0 + 8 * Sh::ROW + at), s[1], z1);
+                uint8_t* at = sm + word_at(q);
+                store_codes4(reinterpret_cast<Code*>(at), s[0], z0);
+                store_codes4(reinterpret_cast<Code*>(at + 8 * Sh::ROW), s[1], z1);
             }
             if (t == 0) {
                 scales[row] = z0.scale;
