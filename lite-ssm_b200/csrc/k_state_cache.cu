@@ -95,14 +95,6 @@ __device__ __forceinline__ void store_codes4(Code* to, const float (&v)[4], cons
     if constexpr (sizeof(Code) == 1) *reinterpret_cast<uint32_t*>(to) = z.sound ? pack_codes8(c) : 0u;
     else *reinterpret_cast<uint2*>(to) = z.sound ? pack_codes16(c) : make_uint2(0u, 0u);
 }
-// max|.| that keeps NaN
-__device__ __forceinline__ float max_nan(float a, float b) { return a != a || b != b ? __int_as_float(0x7FC00000) : fmaxf(a, b); }
-__device__ __forceinline__ float warp_max_nan(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
-
 // Window weights of one head, lane j of a warp for token j (W <= 32): the sum over later tokens
 // is taken from the end, so one very large dt costs the tokens after it no digits.
 __device__ __forceinline__ void window_weights(float a, float dt, uint32_t lane, uint32_t count, float* w, float* alpha) {
@@ -125,9 +117,9 @@ constexpr int SC_THREADS = 256;
 // row, so neighbours are read and written together whatever N and the arrays' alignment are.
 // A step: S_q C of the rows by warps, C . B_j of the window's tokens by warps, then y by a thread a row.
 // A fold or a load: a warp keeps 32 elements of every B_j in registers (KB * 16 of them) and walks down the rows.
-constexpr uint32_t ANY_ROWS = 128;
+constexpr uint32_t ANY_ROWS = 128, ANY_ILP = 8;   // rows at a time; of them, rows a warp has on their way
 template <typename Code, int MODE, int KB>
-__global__ void __launch_bounds__(SC_THREADS) k_state_any(StateCacheArgs a) {
+__global__ void __launch_bounds__(SC_THREADS, KB == 1 ? 3 : 2) k_state_any(StateCacheArgs a) {
     constexpr float Q = sizeof(Code) == 1 ? 127.0f : 32767.0f;
     constexpr int WARPS = SC_THREADS / 32, J = 16 * KB;
     __shared__ __align__(16) float s_xw[ANY_ROWS][J + 4];   // w_j x_j[p], 0 behind the window's tokens
@@ -162,6 +154,7 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_any(StateCacheArgs a) {
         for (uint32_t j = wid; j < count; j += WARPS) {
             const __half* B = token_B(j);
             float d = 0.0f;
+#pragma unroll 4
             for (uint32_t i = lane; i < a.N; i += 32) d = fmaf(__half2float(B[i]), __half2float(Cn[i]), d);
             d = warp_sum(d);
             if (lane == 0) s_cb[j] = d;
@@ -176,6 +169,7 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_any(StateCacheArgs a) {
         if (MODE == 0) {
             for (uint32_t p = wid * 4; p < rows; p += WARPS * 4) {
                 float d[4] = {};
+#pragma unroll 4
                 for (uint32_t i = lane; i < a.N; i += 32) {
                     const float c = __half2float(Cn[i]);
 #pragma unroll
@@ -191,8 +185,13 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_any(StateCacheArgs a) {
             __syncthreads();
             if (tid < rows) {
                 const uint64_t o = (uint64_t)h * a.P + p0 + tid;
+                __half x[J];   // all on their way before the first is used
+#pragma unroll
+                for (uint32_t j = 0; j < J; ++j) x[j] = j < count ? token_x(j)[p0 + tid] : __ushort_as_half(0);
                 float yw = 0.0f;
-                for (uint32_t j = 0; j < count; ++j) yw = fmaf(s_w[j] * s_cb[j], __half2float(token_x(j)[p0 + tid]), yw);
+#pragma unroll
+                for (uint32_t j = 0; j < J; ++j)
+                    if (j < count) yw = fmaf(s_w[j] * s_cb[j], __half2float(x[j]), yw);
                 const __half xh = xn[p0 + tid];
                 const float Dh = a.has_D ? __half2float(a.D[h]) : 0.0f;
                 const __half yh = __float2half_rn(fmaf(alpha * scales[tid], s_row[tid], yw) + Dh * __half2float(xh));
@@ -202,10 +201,9 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_any(StateCacheArgs a) {
             __syncthreads();
             if (!fold) continue;
         }
-        for (uint32_t i = tid; i < rows * J; i += SC_THREADS) {
-            const uint32_t p = i % rows, j = i / rows;
-            s_xw[p][j] = j < count ? s_w[j] * __half2float(token_x(j)[p0 + p]) : 0.0f;
-        }
+        for (uint32_t p = lane; p < rows; p += 32)
+#pragma unroll
+            for (uint32_t j = wid; j < J; j += WARPS) s_xw[p][j] = j < count ? s_w[j] * __half2float(token_x(j)[p0 + p]) : 0.0f;
         if (tid < rows) {
             s_row[tid] = alpha * scales[tid];
             s_top[tid] = 0;
@@ -220,25 +218,24 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_any(StateCacheArgs a) {
                 float B[J];
 #pragma unroll
                 for (uint32_t j = 0; j < J; ++j) B[j] = in && j < count ? __half2float(token_B(j)[i]) : 0.0f;
-                for (uint32_t p = task / chunks * 2; p < rows; p += splits * 2) {
-                    float v[2];
+                for (uint32_t p = task / chunks * ANY_ILP; p < rows; p += splits * ANY_ILP) {
+                    float v[ANY_ILP];
+                    const uint32_t here = min(ANY_ILP, rows - p);
 #pragma unroll
-                    for (uint32_t r = 0; r < 2; ++r) v[r] = in && p + r < rows ? s_row[p + r] * (float)codes[(uint64_t)(p + r) * a.N + i] : 0.0f;
+                    for (uint32_t r = 0; r < ANY_ILP; ++r) v[r] = in && r < here ? (float)codes[(uint64_t)(p + r) * a.N + i] : 0.0f;
 #pragma unroll
-                    for (uint32_t j = 0; j < J; j += 4) {
-                        if (j >= count) break;
+                    for (uint32_t r = 0; r < ANY_ILP; ++r) {
+                        if (r >= here) break;
+                        v[r] *= s_row[p + r];
 #pragma unroll
-                        for (uint32_t r = 0; r < 2; ++r) {
-                            const float4 x = *reinterpret_cast<const float4*>(&s_xw[min(p + r, rows - 1)][j]);
+                        for (uint32_t j = 0; j < J; j += 4) {
+                            if (j >= count) break;
+                            const float4 x = *reinterpret_cast<const float4*>(&s_xw[p + r][j]);
                             v[r] = fmaf(x.x, B[j], v[r]);
                             v[r] = fmaf(x.y, B[j + 1], v[r]);
                             v[r] = fmaf(x.z, B[j + 2], v[r]);
                             v[r] = fmaf(x.w, B[j + 3], v[r]);
                         }
-                    }
-#pragma unroll
-                    for (uint32_t r = 0; r < 2; ++r) {
-                        if (p + r >= rows) break;
                         const uint64_t at = (uint64_t)(p + r) * a.N + i;
                         if constexpr (MODE == 1) {
                             if (in) store_any(a.state, (bh * a.P + p0) * a.N + at, a.state_dtype, v[r]);
@@ -275,7 +272,7 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_any(StateCacheArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-//  N = 128, P a multiple of 16: tensor-core kernel
+//  N = 64, 128 or 256, P a multiple of 16: tensor-core kernel
 // ---------------------------------------------------------------------------
 // A CTA takes `heads` heads of one group and sequence; a warp 16 rows of a head's state at a time. With m16n8k16
 // (f16 in, f32 out), lane
@@ -286,8 +283,8 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_any(StateCacheArgs a) {
 //               the largest at 2^14, B = the window's B; a lane gets the elements whose codes it holds.
 // A code is converted, multiplied and added in about one instruction for 30 elements, so the step is bound by the
 // codes' bytes and the latency of a short CTA.
-constexpr int TC_THREADS = 256, TC_WARPS = TC_THREADS / 32, TC_N = 128, TC_HEADS = 4;
-constexpr uint32_t TC_ROWS = 256;   // rows of 8-bit codes a CTA holds (32 KB)
+constexpr int TC_THREADS = 256, TC_WARPS = TC_THREADS / 32, TC_HEADS = 4;
+constexpr uint32_t TC_BYTES = 32 * 1024;   // of codes a CTA holds (one head may have more)
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -365,34 +362,37 @@ struct Pow2 {
     }
 };
 
-// Shared memory of a CTA: the heads' codes (rows of TC_N, their 16-byte pieces exchanged by row so that neither
+// Shared memory of a CTA: the heads' codes (rows of N, their 16-byte pieces exchanged by row so that neither
 // 16-byte nor 4-byte reads of 8 rows meet in a bank), the window's x (a row a token) and B, C,
 // S_q C of every row, and the pair layout of B.
-template <typename Code, int KB>
+template <typename Code, int KB, int N>
 struct TcShared {
-    static constexpr uint32_t ROW = TC_N * sizeof(Code), PIECES = ROW / 16;
-    static constexpr uint32_t B_PITCH = TC_N * 2 + 16, PAIR_PITCH = TC_N + 16;   // bytes; words
+    static constexpr uint32_t ROW = N * sizeof(Code), PIECES = ROW / 16;
+    static constexpr uint32_t B_PITCH = N * 2 + 16, PAIR_PITCH = N + 16;   // bytes; words
     uint32_t x_pitch, x, B, C, dot, pairs, total;   // bytes from the start; codes are first
     __host__ __device__ TcShared(uint32_t rows) {   // rows: heads * P
         x_pitch = rows * 2 + 16;
         x = rows * ROW;
         B = x + KB * 16 * x_pitch;
         C = B + KB * 16 * B_PITCH;
-        dot = C + TC_N * 2;
+        dot = C + N * 2;
         pairs = dot + rows * 4;
         total = pairs + KB * 8 * PAIR_PITCH * 4;
     }
-    static __device__ __forceinline__ uint32_t swap(uint32_t row) { return (row & 1) << 2 | (row >> 1 & 3); }
+    // rows of 64 bytes lie two to a line of banks; others have a line or more of their own
+    static __device__ __forceinline__ uint32_t swap(uint32_t row) { return PIECES == 4 ? row >> 1 & 3 : (row & 1) << 2 | (row >> 1 & 3); }
     static __device__ __forceinline__ uint32_t piece(uint32_t row, uint32_t i) { return row * ROW + ((i ^ swap(row)) << 4); }
 };
 
 __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
 // KB: blocks of 16 window tokens (W <= 16 * KB). Grid: blocks of heads, groups, sequences.
-template <typename Code, int MODE, int KB>
+// PAD: any N up to the template's and any P, alignment and stride: one head a CTA, read and written element by element,
+// with zeros behind its rows and columns.
+template <typename Code, int MODE, int KB, int N, bool PAD>
 __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_state_tc(StateCacheArgs a, uint32_t heads, uint32_t per_group) {
     constexpr float Q = sizeof(Code) == 1 ? 127.0f : 32767.0f;
-    using Sh = TcShared<Code, KB>;
+    using Sh = TcShared<Code, KB, N>;
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ __align__(16) float s_w[TC_HEADS][32];
     __shared__ __align__(16) float s_cb[MODE == 0 ? 16 * KB : 1];
@@ -400,11 +400,12 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
     const uint32_t first = blockIdx.x * heads, nh = min(heads, per_group - first), b = blockIdx.z;
     const uint32_t h0 = blockIdx.y * per_group + first;   // heads h0 .. h0 + nh - 1
     const uint32_t tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
-    const uint32_t rows = nh * a.P, bh0 = b * a.H + h0;
-    const uint32_t xrow = a.H * a.P, brow = a.G * TC_N;
-    const Sh sh(heads * a.P);
+    const uint32_t real = nh * a.P, rows = PAD ? (a.P + 15) / 16 * 16 : real, bh0 = b * a.H + h0;   // with padding: rows
+    const uint32_t n_real = PAD ? a.N : N, xrow = a.H * a.P, brow = a.G * n_real;
+    const Sh sh(PAD ? rows : heads * a.P);
     const uint32_t sm0 = smem_u32(sm);
-    uint8_t* codes = static_cast<uint8_t*>(a.codes) + (uint64_t)bh0 * a.P * Sh::ROW;
+    Code* const g_codes = static_cast<Code*>(a.codes) + (uint64_t)bh0 * a.P * n_real;
+    uint8_t* codes = reinterpret_cast<uint8_t*>(g_codes);
     float* scales = a.scales + (uint64_t)bh0 * a.P;
     const uint32_t filled = a.fill[bh0];
     // what warp w < nh needs for head w's weights, and this thread's row
@@ -420,8 +421,14 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
             if (a.has_D) p_D = a.D[h];
         }
     }
-    const float my_scale = tid < rows ? scales[tid] : 0.0f;
-    {
+    const float my_scale = tid < real ? scales[tid] : 0.0f;
+    auto code_at = [&](uint32_t row, uint32_t e) { return Sh::piece(row, e * sizeof(Code) >> 4) + (e * sizeof(Code) & 15); };
+    if constexpr (PAD) {
+        for (uint32_t r = wid; r < rows; r += TC_WARPS)
+#pragma unroll
+            for (uint32_t e = lane; e < N; e += 32)
+                *reinterpret_cast<Code*>(sm + code_at(r, e)) = r < real && e < n_real ? g_codes[r * n_real + e] : (Code)0;
+    } else {
         const uint8_t* from = codes + tid * 16;
         constexpr uint32_t STEP = TC_THREADS / Sh::PIECES;   // rows a round, a multiple of 8: the exchange repeats
         uint32_t to = sm0 + Sh::piece(tid / Sh::PIECES, tid % Sh::PIECES);
@@ -431,12 +438,27 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
     const uint32_t n = MODE == 0 ? min(filled, a.W - 1) : a.W, count = MODE == 0 ? n + 1 : min(filled, a.W);
     const bool fold = MODE == 0 && count == a.W;
     const __half* wx = a.win_x + ((uint64_t)b * a.W * xrow + (uint64_t)h0 * a.P);
-    __half* wB = a.win_B + ((uint64_t)b * a.W * brow + blockIdx.y * TC_N);
+    __half* wB = a.win_B + ((uint64_t)b * a.W * brow + blockIdx.y * n_real);
     const __half* xn = MODE == 0 ? a.x + b * a.x_bs + (uint64_t)h0 * a.P : nullptr;
-    const __half* Bn = MODE == 0 ? a.B + b * a.bc_bs + blockIdx.y * TC_N : nullptr;
-    // the window's rows, a warp each of x, half a warp each of B; those behind its tokens are zeros, so that their
+    const __half* Bn = MODE == 0 ? a.B + b * a.bc_bs + blockIdx.y * n_real : nullptr;
+    const __half* Cn = MODE == 0 ? a.C + b * a.bc_bs + blockIdx.y * n_real : nullptr;
+    // the window's rows, a warp each of x; those behind its tokens are zeros, so that their
     // products are
-    if (MODE == 0 || count) {
+    if constexpr (PAD) {
+        const __half zero = __ushort_as_half(0);
+        if (MODE == 0 || count)
+            for (uint32_t j = wid; j < KB * 16; j += TC_WARPS) {
+                const __half* xj = MODE == 0 && j == n ? xn : wx + (uint64_t)j * xrow;
+                const __half* Bj = MODE == 0 && j == n ? Bn : wB + (uint64_t)j * brow;
+#pragma unroll 4
+                for (uint32_t e = lane; e < rows; e += 32)
+                    *reinterpret_cast<__half*>(sm + sh.x + j * sh.x_pitch + e * 2) = j < count && e < real ? xj[e] : zero;
+#pragma unroll
+                for (uint32_t e = lane; e < N; e += 32)
+                    *reinterpret_cast<__half*>(sm + sh.B + j * Sh::B_PITCH + e * 2) = j < count && e < n_real ? Bj[e] : zero;
+            }
+        if (MODE == 0 && tid < N) *reinterpret_cast<__half*>(sm + sh.C + tid * 2) = tid < n_real ? Cn[tid] : zero;
+    } else if (MODE == 0 || count) {
         for (uint32_t j = wid; j < KB * 16; j += TC_WARPS) {
             const __half* from = MODE == 0 && j == n ? xn : wx + (uint64_t)j * xrow;
             const uint32_t to = sh.x + j * sh.x_pitch;
@@ -446,13 +468,13 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
             }
         }
 #pragma unroll
-        for (uint32_t k = 0; k < KB; ++k) {
-            const uint32_t j = 16 * k + tid / 16, e = tid % 16, to = sh.B + j * Sh::B_PITCH + e * 16;
+        for (uint32_t i = tid; i < KB * 16 * (N / 8); i += TC_THREADS) {
+            const uint32_t j = i / (N / 8), e = i % (N / 8), to = sh.B + j * Sh::B_PITCH + e * 16;
             if (j < count) copy_async16(sm0 + to, (MODE == 0 && j == n ? Bn : wB + (uint64_t)j * brow) + e * 8);
             else *reinterpret_cast<uint4*>(sm + to) = make_uint4(0, 0, 0, 0);
         }
     }
-    if (MODE == 0 && tid < TC_N / 8) copy_async16(sm0 + sh.C + tid * 16, a.C + b * a.bc_bs + blockIdx.y * TC_N + tid * 8);
+    if (!PAD && MODE == 0 && tid < N / 8) copy_async16(sm0 + sh.C + tid * 16, Cn + tid * 8);
     if (wid < nh) {
         float dt = lane < count ? p_dt : 0.0f;
         if (MODE == 0 && lane == n) dt = token_dt(__half2float(p_raw) + __half2float(p_bias), a.dt_min, a.dt_max);
@@ -468,8 +490,8 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
     if (MODE == 1 ? count > 0 : fold) {
         // tokens 2 jp and 2 jp + 1 of the window's B side by side, as the product wants them
 #pragma unroll
-        for (uint32_t i = tid; i < KB * 8 * (TC_N / 2); i += TC_THREADS) {
-            const uint32_t jp = i / (TC_N / 2), e = i % (TC_N / 2) * 2;
+        for (uint32_t i = tid; i < KB * 8 * (N / 2); i += TC_THREADS) {
+            const uint32_t jp = i / (N / 2), e = i % (N / 2) * 2;
             const uint8_t* from = sm + sh.B + 2 * jp * Sh::B_PITCH + e * 2;
             const uint32_t p0 = *reinterpret_cast<const uint32_t*>(from), p1 = *reinterpret_cast<const uint32_t*>(from + Sh::B_PITCH);
             // of every four elements in the order 0, 2, 1, 3: a lane uses 0 and 2, or 1 and 3, of them
@@ -489,7 +511,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
             // 16 bytes a row and lane at a time, piece 4 i + t
             float lo[2][4] = {}, hi[2][4] = {};
 #pragma unroll
-            for (int i = 0; i < (int)(8 * sizeof(Code) / 4); ++i) {
+            for (int i = 0; i < (int)Sh::PIECES / 4; ++i) {
                 const uint32_t at = ((4 * i + t) ^ sw) << 4;
                 const uint4 u4 = lds16(r0 + at), v4 = lds16(r0 + 8 * Sh::ROW + at);
                 const uint32_t u[4] = {u4.x, u4.y, u4.z, u4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
@@ -530,7 +552,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
             const uint32_t j0 = 16 * (TC_WARPS - 1 - wid) + g;
             const uint8_t* r0 = sm + sh.B + j0 * Sh::B_PITCH + 16 * t;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < N / 32; ++i) {
                 const uint4 p0 = lds16(r0 + 64 * i), p1 = lds16(r0 + 8 * Sh::B_PITCH + 64 * i), c = lds16(sm + sh.C + 64 * i + 16 * t);
                 mma16816(d, p0.x, p1.x, p0.y, p1.y, c.x, c.y);
                 mma16816(d, p0.z, p1.z, p0.w, p1.w, c.z, c.w);
@@ -539,8 +561,8 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
         }
         __syncthreads();
         // y: a thread a row
-        if (tid < rows) {
-            const uint32_t hh = head_of(tid);
+        if (tid < real) {
+            const uint32_t hh = PAD ? 0 : head_of(tid);
             const __half* x = reinterpret_cast<const __half*>(sm + sh.x) + tid;
             const float* w = s_w[hh];
             float yw = 0.0f;
@@ -560,18 +582,21 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
             a.win_x[((uint64_t)b * a.W + n) * xrow + o] = xh;
         }
         // the first head of a group keeps the group's B row; every head takes row n from its argument
-        if (first == 0 && tid < TC_N / 8)
+        if (PAD) {
+            if (first == 0 && tid < n_real) wB[(uint64_t)n * brow + tid] = *reinterpret_cast<const __half*>(sm + sh.B + n * Sh::B_PITCH + tid * 2);
+        } else if (first == 0 && tid < N / 8) {
             *reinterpret_cast<uint4*>(wB + (uint64_t)n * brow + 8 * tid) = lds16(sm + sh.B + n * Sh::B_PITCH + 16 * tid);
+        }
         if (tid < nh) a.fill[bh0 + tid] = fold ? 0 : count;
         if (!fold) return;
     }
     float* s_as = reinterpret_cast<float*>(sm + sh.dot);   // alpha * scale of every row
     if (MODE == 0) __syncthreads();
-    if (tid < rows) s_as[tid] = s_alpha[head_of(tid)] * my_scale;
+    if (tid < rows) s_as[tid] = tid < real ? s_alpha[PAD ? 0 : head_of(tid)] * my_scale : 0.0f;
     __syncthreads();
     const uint32_t ldm = sm0 + sh.x + ((lane & 7) + (lane >> 4 & 1) * 8) * sh.x_pitch + (lane >> 3 & 1) * 16;
     for (uint32_t tile = wid; tile < rows / 16; tile += TC_WARPS) {
-        const uint32_t row = tile * 16 + g, hh = head_of(tile * 16), sw = Sh::swap(row);   // of row + 8, too
+        const uint32_t row = tile * 16 + g, hh = PAD ? 0 : head_of(tile * 16), sw = Sh::swap(row);   // of row + 8, too
         const float as[2] = {s_as[row], s_as[row + 8]};
         // w_j x_j[p] of the lane's tokens: [0], [1] row g, tokens 2t, 2t + 1; [2], [3] row g + 8; [4] .. [7] tokens + 8
         float xw[KB * 8];
@@ -629,15 +654,22 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
             }
         };
         if constexpr (MODE == 1) {
-            const uint64_t o0 = ((uint64_t)bh0 * a.P + row) * TC_N + 4 * t;
+            const uint64_t o0 = ((uint64_t)bh0 * a.P + row) * n_real + 4 * t;
+            // padded rows and columns are left out; without them, stores of four where the state's rows allow it
+            const bool wide = !PAD || (a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.state) & 15) == 0);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
+            for (int q = 0; q < N / 16; ++q) {
                 float s[2][4];
                 word(q, s);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const uint64_t o = o0 + 8 * TC_N * r + 16 * q;
-                    if (a.state_dtype == LSSM_DT_F32)
+                    const uint64_t o = o0 + 8 * n_real * r + 16 * q;
+                    if (PAD && (row + 8 * r >= real || 16 * q + 4 * t >= n_real)) continue;
+                    if (PAD && !wide) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i)
+                            if (16 * q + 4 * t + i < n_real) store_any(a.state, o + i, a.state_dtype, s[r][i]);
+                    } else if (a.state_dtype == LSSM_DT_F32)
                         __stcs(reinterpret_cast<float4*>(static_cast<float*>(a.state) + o), make_float4(s[r][0], s[r][1], s[r][2], s[r][3]));
                     else {
                         uint2 w;
@@ -657,7 +689,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
             // holds the registers for it.
             float amax[2] = {};
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
+            for (int q = 0; q < N / 16; ++q) {
                 float s[2][4];
                 word(q, s);
 #pragma unroll
@@ -669,7 +701,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
                 for (int r = 0; r < 2; ++r) amax[r] = max_keep_nan(amax[r], __shfl_xor_sync(0xffffffffu, amax[r], o));
             const RowQuant z0(amax[0], Q), z1(amax[1], Q);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
+            for (int q = 0; q < N / 16; ++q) {
                 float s[2][4];
                 word(q, s);
                 uint8_t* at = sm + word_at(q);
@@ -677,11 +709,14 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
                 store_codes4(reinterpret_cast<Code*>(at + 8 * Sh::ROW), s[1], z1);
             }
             if (t == 0) {
-                scales[row] = z0.scale;
-                scales[row + 8] = z1.scale;
+                if (!PAD || row < real) scales[row] = z0.scale;
+                if (!PAD || row + 8 < real) scales[row + 8] = z1.scale;
             }
             __syncwarp();
-            for (uint32_t i = lane; i < 16 * Sh::PIECES; i += 32) {
+            if constexpr (PAD) {
+                for (uint32_t r = tile * 16; r < min(tile * 16 + 16, real); ++r)
+                    for (uint32_t e = lane; e < n_real; e += 32) g_codes[r * n_real + e] = *reinterpret_cast<const Code*>(sm + code_at(r, e));
+            } else for (uint32_t i = lane; i < 16 * Sh::PIECES; i += 32) {
                 const uint32_t rr = tile * 16 + i / Sh::PIECES, q = i % Sh::PIECES;
                 *reinterpret_cast<uint4*>(codes + rr * Sh::ROW + q * 16) = lds16(sm + Sh::piece(rr, q));
             }
@@ -689,36 +724,46 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
     }
 }
 
-template <typename Code, int MODE, int KB>
-cudaError_t launch_tc(const StateCacheArgs& a, uint32_t heads, cudaStream_t s) {
-    const uint32_t bytes = TcShared<Code, KB>(heads * a.P).total;
+template <typename Code, int MODE, int KB, int N, bool PAD>
+cudaError_t launch_tc(const StateCacheArgs& a, cudaStream_t s) {
+    // Heads of a group share the window's B and what is computed from it: as many as TC_BYTES of codes allow, fewer
+    // where the grid would leave SMs without a CTA.
+    const uint32_t per_group = a.H / a.G;
+    uint32_t heads = PAD ? 1 : TC_HEADS;
+    while (heads > 1 && (heads * a.P > TC_THREADS || heads * a.P * N * sizeof(Code) > TC_BYTES ||
+                         (uint64_t)a.batch * a.G * ((per_group + heads - 1) / heads) < 2ull * 148)) heads /= 2;
+    const uint32_t bytes = TcShared<Code, KB, N>(PAD ? (a.P + 15) / 16 * 16 : heads * a.P).total;
+    const auto kernel = k_state_tc<Code, MODE, KB, N, PAD>;
     if (bytes > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(k_state_tc<Code, MODE, KB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         if (e != cudaSuccess) return e;
     }
-    const uint32_t per_group = a.H / a.G;
-    k_state_tc<Code, MODE, KB><<<dim3((per_group + heads - 1) / heads, a.G, a.batch), TC_THREADS, bytes, s>>>(a, heads, per_group);
+    kernel<<<dim3((per_group + heads - 1) / heads, a.G, a.batch), TC_THREADS, bytes, s>>>(a, heads, per_group);
     return cudaGetLastError();
+}
+template <typename Code, int MODE, int N, bool PAD>
+cudaError_t launch_tc_of(const StateCacheArgs& a, cudaStream_t s) {
+    return a.W <= 16 ? launch_tc<Code, MODE, 1, N, PAD>(a, s) : launch_tc<Code, MODE, 2, N, PAD>(a, s);
 }
 
 template <typename Code, int MODE>
 cudaError_t launch_cached(const StateCacheArgs& a, cudaStream_t s) {
-    // rows of 128 and heads of 16 rows keep the arrays' 16-byte alignment
-    bool tc = a.N == TC_N && a.P % 16 == 0 && a.P <= TC_ROWS && a.G <= 65535 && a.batch <= 65535 && aligned(a.codes, 16) && aligned(a.win_x, 16) && aligned(a.win_B, 16);
-    if (MODE == 0) tc = tc && aligned(a.x, 16) && aligned(a.B, 16) && aligned(a.C, 16) && a.bc_bs % 8 == 0 && a.x_bs % 8 == 0;
-    else tc = tc && aligned(a.state, 16);
-    if (!tc) {
-        if (a.W <= 16) k_state_any<Code, MODE, 1><<<a.batch * a.H, SC_THREADS, 0, s>>>(a);
-        else k_state_any<Code, MODE, 2><<<a.batch * a.H, SC_THREADS, 0, s>>>(a);
-        return cudaGetLastError();
+    // a thread has a row
+    if (a.P <= TC_THREADS && a.N <= 256 && a.G <= 65535 && a.batch <= 65535) {
+        // such rows, and heads of 16 rows, keep the arrays' 16-byte alignment
+        bool whole = a.P % 16 == 0 && aligned(a.codes, 16) && aligned(a.win_x, 16) && aligned(a.win_B, 16);
+        if (MODE == 0) whole = whole && aligned(a.x, 16) && aligned(a.B, 16) && aligned(a.C, 16) && a.bc_bs % 8 == 0 && a.x_bs % 8 == 0;
+        else whole = whole && aligned(a.state, 16);
+        if (whole && a.N == 128) return launch_tc_of<Code, MODE, 128, false>(a, s);
+        if (whole && a.N == 64) return launch_tc_of<Code, MODE, 64, false>(a, s);
+        if (whole && a.N == 256) return launch_tc_of<Code, MODE, 256, false>(a, s);
+        if (a.N <= 64) return launch_tc_of<Code, MODE, 64, true>(a, s);
+        if (a.N <= 128) return launch_tc_of<Code, MODE, 128, true>(a, s);
+        return launch_tc_of<Code, MODE, 256, true>(a, s);
     }
-    // Heads of a group share the window's B and what is computed from it: as many as 32 KB of codes allow, fewer
-    // where the grid would leave SMs without a CTA.
-    const uint32_t per_group = a.H / a.G;
-    uint32_t heads = TC_HEADS;
-    while (heads > 1 && (heads * a.P > TC_ROWS / sizeof(Code) ||
-                         (uint64_t)a.batch * a.G * ((per_group + heads - 1) / heads) < 2ull * 148)) heads /= 2;
-    return a.W <= 16 ? launch_tc<Code, MODE, 1>(a, heads, s) : launch_tc<Code, MODE, 2>(a, heads, s);
+    if (a.W <= 16) k_state_any<Code, MODE, 1><<<a.batch * a.H, SC_THREADS, 0, s>>>(a);
+    else k_state_any<Code, MODE, 2><<<a.batch * a.H, SC_THREADS, 0, s>>>(a);
+    return cudaGetLastError();
 }
 
 template <typename Code>
@@ -729,9 +774,12 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_store(StateCacheArgs a) {
     if (row >= rows) return;
     const float* S = static_cast<const float*>(a.state) + row * a.N;
     Code* out = static_cast<Code*>(a.codes) + row * a.N;
-    float amax = 0.0f;
-    for (uint32_t i = lane; i < a.N; i += 32) amax = max_nan(amax, fabsf(S[i]));
-    const RowQuant z(warp_max_nan(amax), Q);
+    // the bits of |v| order as the values do, NaN above infinity
+    uint32_t top = 0;
+#pragma unroll 8
+    for (uint32_t i = lane; i < a.N; i += 32) top = max(top, __float_as_uint(S[i]) & 0x7FFFFFFFu);
+    const RowQuant z(__uint_as_float(__reduce_max_sync(0xffffffffu, top)), Q);
+#pragma unroll 4
     for (uint32_t i = lane; i < a.N; i += 32) out[i] = quantise1<Code>(S[i], z);
     if (lane == 0) {
         a.scales[row] = z.scale;
