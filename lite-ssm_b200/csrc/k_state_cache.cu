@@ -734,7 +734,7 @@ cudaError_t launch_tc(const StateCacheArgs& a, cudaStream_t s) {
                          (uint64_t)a.batch * a.G * ((per_group + heads - 1) / heads) < 2ull * 148)) heads /= 2;
     const uint32_t bytes = TcShared<Code, KB, N>(PAD ? (a.P + 15) / 16 * 16 : heads * a.P).total;
     const auto kernel = k_state_tc<Code, MODE, KB, N, PAD>;
-    if (bytes > 48 * 1024) {
+    if (bytes > 36 * 1024) {   // with the static part, more than 48 KB
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         if (e != cudaSuccess) return e;
     }
@@ -787,44 +787,79 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_store(StateCacheArgs a) {
     }
 }
 
-// N = 128: a warp takes STORE_ROWS rows, a lane four neighbours of each. The largest magnitude is found on the
-// bits of |v|, which order as the values do, with NaN above infinity.
-constexpr int STORE_ROWS = 8;
-template <typename Code>
-__global__ void __launch_bounds__(SC_THREADS) k_state_store128(StateCacheArgs a) {
+// N up to 256: a warp takes ROWS rows, a lane PER elements of each in registers: VEC neighbours at a time (VEC 4: N a
+// multiple of 4 and the arrays aligned for it), runs of 32 * VEC. Lane r works out row r's scale. The largest magnitude
+// is found on the bits of |v|, which order as the values do, with NaN above infinity.
+template <typename Code, int ROWS, int PER, int VEC>
+__global__ void __launch_bounds__(SC_THREADS) k_state_store_rows(StateCacheArgs a) {
     constexpr float Q = sizeof(Code) == 1 ? 127.0f : 32767.0f;
     const uint32_t lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-    const uint64_t row0 = ((uint64_t)blockIdx.x * (SC_THREADS / 32) + wid) * STORE_ROWS, rows = (uint64_t)a.batch * a.H * a.P;
-    const float* S = static_cast<const float*>(a.state) + row0 * 128 + 4 * lane;
-    Code* out = static_cast<Code*>(a.codes) + row0 * 128 + 4 * lane;
-    float4 v[STORE_ROWS];
+    const uint64_t row0 = ((uint64_t)blockIdx.x * (SC_THREADS / 32) + wid) * ROWS, rows = (uint64_t)a.batch * a.H * a.P;
+    if (row0 >= rows) return;
+    const uint32_t here = (uint32_t)(rows - row0 < ROWS ? rows - row0 : ROWS);
+    const float* S = static_cast<const float*>(a.state) + row0 * a.N;
+    Code* out = static_cast<Code*>(a.codes) + row0 * a.N;
+    float v[ROWS][PER];
 #pragma unroll
-    for (int r = 0; r < STORE_ROWS; ++r)
-        if (row0 + r < rows) v[r] = __ldcs(reinterpret_cast<const float4*>(S + r * 128));
-    // lane r works out row r's scale
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int k = 0; k < PER; k += VEC) {
+            const uint32_t e = k * 32 + lane * VEC;
+            const bool in = r < (int)here && e < a.N;
+            if constexpr (VEC == 4) {
+                const float4 f = in ? __ldcs(reinterpret_cast<const float4*>(S + r * a.N + e)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                v[r][k] = f.x; v[r][k + 1] = f.y; v[r][k + 2] = f.z; v[r][k + 3] = f.w;
+            } else v[r][k] = in ? __ldcs(S + r * a.N + e) : 0.0f;
+        }
     uint32_t mine = 0;
 #pragma unroll
-    for (int r = 0; r < STORE_ROWS; ++r) {
+    for (int r = 0; r < ROWS; ++r) {
         uint32_t top = 0;
-        if (row0 + r < rows) {
-            const float e[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(e[i]) & 0x7FFFFFFFu);
-        }
+        for (int k = 0; k < PER; ++k) top = max(top, __float_as_uint(v[r][k]) & 0x7FFFFFFFu);
         top = __reduce_max_sync(0xffffffffu, top);
         if ((int)lane == r) mine = top;
     }
     const RowQuant own(__uint_as_float(mine), Q);
 #pragma unroll
-    for (int r = 0; r < STORE_ROWS; ++r) {
-        if (row0 + r >= rows) break;
-        const float e[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
-        store_codes4(out + r * 128, e, own.of_lane(r));
+    for (int r = 0; r < ROWS; ++r) {
+        const RowQuant z = own.of_lane(r);
+#pragma unroll
+        for (int k = 0; k < PER; k += 4) {
+            const float four[4] = {v[r][k], v[r][k + 1], v[r][k + 2], v[r][k + 3]};
+            if constexpr (VEC == 4) {
+                const uint32_t e = k * 32 + lane * 4;
+                if (r < (int)here && e < a.N) store_codes4(out + r * a.N + e, four, z);
+            } else {
+                uint32_t c[4];
+                quantise4(four, z, c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t e = (k + i) * 32 + lane;
+                    if (r < (int)here && e < a.N) out[r * a.N + e] = z.sound ? (Code)c[i] : (Code)0;
+                }
+            }
+        }
     }
-    if (lane < STORE_ROWS && row0 + lane < rows) {
+    if (lane < here) {
         a.scales[row0 + lane] = own.scale;
         if ((row0 + lane) % a.P == 0) a.fill[(row0 + lane) / a.P] = 0;
     }
+}
+template <typename Code, int ROWS, int PER>
+void launch_store_rows(const StateCacheArgs& a, uint64_t rows, cudaStream_t s) {
+    constexpr uint64_t EACH = SC_THREADS / 32 * ROWS;
+    const unsigned grid = (unsigned)((rows + EACH - 1) / EACH);
+    if (a.N % 4 == 0 && aligned(a.state, 16) && aligned(a.codes, 4 * sizeof(Code))) k_state_store_rows<Code, ROWS, PER, 4><<<grid, SC_THREADS, 0, s>>>(a);
+    else k_state_store_rows<Code, ROWS, PER, 1><<<grid, SC_THREADS, 0, s>>>(a);
+}
+template <typename Code>
+cudaError_t launch_store_of(const StateCacheArgs& a, uint64_t rows, cudaStream_t s) {
+    // 32 elements a lane in flight
+    if (a.N <= 128) launch_store_rows<Code, 8, 4>(a, rows, s);
+    else if (a.N <= 256) launch_store_rows<Code, 4, 8>(a, rows, s);
+    else k_state_store<Code><<<(unsigned)((rows + SC_THREADS / 32 - 1) / (SC_THREADS / 32)), SC_THREADS, 0, s>>>(a);
+    return cudaGetLastError();
 }
 
 }  // namespace
@@ -832,17 +867,7 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_store128(StateCacheArgs a)
 cudaError_t launch_state_store(const StateCacheArgs& a, cudaStream_t s) {
     const uint64_t rows = (uint64_t)a.batch * a.H * a.P;
     if (!rows || !a.N) return cudaSuccess;
-    if (a.N == 128 && aligned(a.state, 16) && aligned(a.codes, 8)) {
-        constexpr unsigned PER = SC_THREADS / 32 * STORE_ROWS;
-        const unsigned grid = (unsigned)((rows + PER - 1) / PER);
-        if (a.bits == 8) k_state_store128<int8_t><<<grid, SC_THREADS, 0, s>>>(a);
-        else k_state_store128<int16_t><<<grid, SC_THREADS, 0, s>>>(a);
-        return cudaGetLastError();
-    }
-    const unsigned grid = (unsigned)((rows + SC_THREADS / 32 - 1) / (SC_THREADS / 32));
-    if (a.bits == 8) k_state_store<int8_t><<<grid, SC_THREADS, 0, s>>>(a);
-    else k_state_store<int16_t><<<grid, SC_THREADS, 0, s>>>(a);
-    return cudaGetLastError();
+    return a.bits == 8 ? launch_store_of<int8_t>(a, rows, s) : launch_store_of<int16_t>(a, rows, s);
 }
 
 cudaError_t launch_state_load(const StateCacheArgs& a, cudaStream_t s) {

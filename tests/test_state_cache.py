@@ -236,7 +236,12 @@ def run_tokens(c, rng, tokens, check_every=1):
 # (batch, H, P, N, G, window): the common shape; odd and tiny ones; several groups; W = 1 and 32
 SHAPES = [(3, 4, 64, 128, 1, 16), (1, 24, 64, 128, 1, 16), (2, 8, 64, 128, 4, 5), (2, 3, 64, 128, 1, 32), (1, 2, 64, 128, 1, 1),
           (2, 2, 16, 128, 2, 17), (1, 1, 1, 1, 1, 1), (2, 6, 5, 7, 3, 3), (1, 3, 48, 75, 1, 8), (2, 2, 33, 300, 1, 4), (1, 5, 128, 256, 5, 16),
-          (2, 4, 80, 128, 2, 12), (1, 3, 64, 64, 1, 16), (65, 2, 64, 128, 1, 4)]
+          (2, 4, 80, 128, 2, 12), (1, 3, 64, 64, 1, 16), (65, 2, 64, 128, 1, 4),
+          # the other state sizes with whole rows, long windows; rows padded to 64, 128 and 256 columns; the most
+          # shared memory; more rows or columns than the padded kernel holds
+          (2, 4, 64, 64, 2, 21), (3, 3, 128, 256, 1, 32), (40, 8, 16, 64, 1, 3), (2, 3, 75, 203, 1, 16), (2, 2, 31, 100, 1, 30),
+          (1, 2, 255, 255, 1, 20), (1, 1, 256, 256, 1, 5), (1, 2, 300, 40, 1, 3), (1, 2, 20, 260, 2, 18), (1, 1, 257, 261, 1, 32),
+          (2, 1, 4, 36, 1, 2)]
 
 
 @pytest.mark.gpu
