@@ -564,7 +564,9 @@ lssm_status lssm_ssd_step_batched(lssm_ctx* ctx, const void* x, const void* B, c
 
 // ---- scoring ----------------------------------------------------------------
 // The checks of these ops need no device: they come before the context is looked at.
-static bool stride_bad(uint64_t stride, uint32_t n) { return stride && (stride < n || stride > (1ull << 40)); }
+static bool stride_bad(uint64_t stride, uint32_t n, uint32_t rows) {
+    return stride && (stride < n || stride > (1ull << 40) || (uint64_t)rows > (1ull << 56) / stride);
+}
 static size_t dtype_bytes(uint32_t dt) { return dt == LSSM_DT_F32 ? 4 : 2; }
 
 lssm_status lssm_logprobs(lssm_ctx* ctx, const void* logits, const uint32_t* targets, float* logp, float* entropy,
@@ -575,8 +577,8 @@ lssm_status lssm_logprobs(lssm_ctx* ctx, const void* logits, const uint32_t* tar
     if (d.rows > 0x7FFFFFFFu) return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: rows must be below 2^31");
     if (d.top_k > LSSM_TOP_K_MAX || d.top_k > d.vocab)
         return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: top_k must be at most %u and at most vocab", LSSM_TOP_K_MAX);
-    if (stride_bad(d.row_stride, d.vocab))
-        return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: row_stride must be 0 or vocab .. 2^40");
+    if (stride_bad(d.row_stride, d.vocab, d.rows))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: row_stride must be 0 or vocab .. 2^40 (rows * row_stride below 2^56)");
     if ((top_ids != nullptr) != (d.top_k > 0) || (top_logp != nullptr) != (d.top_k > 0))
         return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: top_ids and top_logp are given exactly when top_k > 0");
     if (!logp && !entropy && !lse && !d.top_k) return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs: no output given");
@@ -604,8 +606,8 @@ lssm_status lssm_logprobs_backward(lssm_ctx* ctx, const void* logits, const uint
     if (d.vocab == 0 || d.vocab > 0x7FFFFFFFu)
         return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: vocab must be 1 .. 2^31 - 1");
     if (d.rows > 0x7FFFFFFFu) return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: rows must be below 2^31");
-    if (stride_bad(d.row_stride, d.vocab) || stride_bad(d.grad_stride, d.vocab))
-        return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: row_stride and grad_stride must be 0 or vocab .. 2^40");
+    if (stride_bad(d.row_stride, d.vocab, d.rows) || stride_bad(d.grad_stride, d.vocab, d.rows))
+        return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: row_stride and grad_stride must be 0 or vocab .. 2^40 (times rows below 2^56)");
     if (!g_logp && !g_entropy) return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: no gradient given");
     if (d.rows && (!logits || !lse || !dlogits))
         return fail(LSSM_ERR_INVALID_ARGUMENT, "logprobs_backward: null logits, lse or dlogits");
@@ -647,6 +649,7 @@ static lssm_status state_cache_checks(const char* who, const lssm_state_cache_di
     return LSSM_OK;
 }
 
+static bool state_cache_empty(const lssm_state_cache_dims& d) { return !d.batch || !d.H || !d.P || !d.N; }
 static lssm_status state_cache_args(const char* who, const lssm_state_cache& c, const lssm_state_cache_dims& d,
                                     StateCacheArgs* a) {
     if (!c.codes || !c.scales || !c.win_x || !c.win_B || !c.win_dt || !c.fill)
@@ -680,13 +683,16 @@ lssm_status lssm_state_cache_bytes(lssm_state_cache_dims d, uint64_t* out) {
 lssm_status lssm_state_cache_store(lssm_ctx* ctx, const float* state, lssm_state_cache cache,
                                    lssm_state_cache_dims d) {
     if (lssm_status st = state_cache_checks("state_cache_store", d)) return st;
+    if (state_cache_empty(d)) {
+        CHECK_CTX(ctx);
+        return finish_op(ctx, "state_cache_store");
+    }
     StateCacheArgs a;
     if (lssm_status st = state_cache_args("state_cache_store", cache, d, &a)) return st;
     if (!state || !aligned(state, 4))
         return fail(LSSM_ERR_INVALID_ARGUMENT, "state_cache_store: null or misaligned state");
     a.state = const_cast<float*>(state);
     CHECK_CTX(ctx);
-    if (!d.batch || !d.H || !d.P || !d.N) return finish_op(ctx, "state_cache_store");
     LAUNCH("state_cache_store", launch_state_store(a, ctx->stream));
 }
 
@@ -694,6 +700,10 @@ lssm_status lssm_state_cache_load(lssm_ctx* ctx, lssm_state_cache cache, const v
                                   uint32_t state_dtype, lssm_state_cache_dims d) {
     if (lssm_status st = state_cache_checks("state_cache_load", d)) return st;
     if (state_dtype > LSSM_DT_F32) return fail(LSSM_ERR_INVALID_ARGUMENT, "state_cache_load: unsupported dtype code");
+    if (state_cache_empty(d)) {
+        CHECK_CTX(ctx);
+        return finish_op(ctx, "state_cache_load");
+    }
     StateCacheArgs a;
     if (lssm_status st = state_cache_args("state_cache_load", cache, d, &a)) return st;
     if (!state || !aligned(state, dtype_bytes(state_dtype)) || !A_log || !aligned(A_log, 2))
@@ -701,7 +711,6 @@ lssm_status lssm_state_cache_load(lssm_ctx* ctx, lssm_state_cache cache, const v
     a.A_log = static_cast<const __half*>(A_log);
     a.state = state; a.state_dtype = state_dtype;
     CHECK_CTX(ctx);
-    if (!d.batch || !d.H || !d.P || !d.N) return finish_op(ctx, "state_cache_load");
     LAUNCH("state_cache_load", launch_state_load(a, ctx->stream));
 }
 
@@ -709,6 +718,10 @@ lssm_status lssm_ssd_step_cached(lssm_ctx* ctx, const void* x, const void* B, co
                                  const void* dt_bias, const void* A_log, const void* D_skip, lssm_state_cache cache,
                                  void* y, lssm_state_cache_dims d) {
     if (lssm_status st = state_cache_checks("ssd_step_cached", d)) return st;
+    if (state_cache_empty(d)) {
+        CHECK_CTX(ctx);
+        return finish_op(ctx, "ssd_step_cached");
+    }
     StateCacheArgs a;
     if (lssm_status st = state_cache_args("ssd_step_cached", cache, d, &a)) return st;
     if (!x || !B || !C || !dt_raw || !dt_bias || !A_log || !y || (d.has_D && !D_skip))
@@ -722,7 +735,6 @@ lssm_status lssm_ssd_step_cached(lssm_ctx* ctx, const void* x, const void* B, co
     a.y = static_cast<__half*>(y);
     a.x_bs = (uint64_t)d.H * d.P; a.bc_bs = (uint64_t)a.G * d.N; a.dt_bs = d.H; a.y_bs = a.x_bs;
     CHECK_CTX(ctx);
-    if (!d.batch || !d.H || !d.P || !d.N) return finish_op(ctx, "ssd_step_cached");
     LAUNCH("ssd_step_cached", launch_ssd_step_cached(a, ctx->stream));
 }
 

@@ -706,11 +706,12 @@ cudaError_t launch_grad_of(const LogprobsGradArgs& a, cudaStream_t s) {
 
 cudaError_t launch_logprobs(const LogprobsArgs& a, cudaStream_t s) {
     if (!a.rows) return cudaSuccess;
-    // A few long rows: a cluster of CTAs a row. A cluster costs its launch and its join: slices below 32 K entries
-    // and more than about two CTAs an SM lose by it (256000 fp16 entries, top 5: 1 row 20.1 us with one CTA, 9.2
-    // with 8; 64 rows 28.0 / 18.5 / 14.4 / 16.5 with 1 / 2 / 4 / 8; 50288 entries, 128 rows 10.1 / 10.3 / 12.5).
+    // A few long rows: a cluster of CTAs a row. A cluster costs its join and the CTAs' own ends: slices below 32 K
+    // entries and more than about three CTAs an SM lose by it (with 1 / 2 / 4 / 8 CTAs a row: 1 row of 256000 fp16,
+    // top 5, 20.1 / 14.4 / 10.3 / 8.9 us; 64 rows 28.7 / 18.6 / 14.4 / 16.5; 333 rows of 32001 fp32, top 8,
+    // 14.4 / 20.6 / 23.2 / 37.2; 128 rows of 50288 fp16, top 20, 10.1 / 10.3 / 12.5 / 18.7).
     uint32_t nc = 1;
-    while (nc < LP_CLUSTER_MAX && (uint64_t)a.rows * nc * 2 <= 400 && a.vocab / (nc * 2) >= 32000) nc *= 2;
+    while (nc < LP_CLUSTER_MAX && (uint64_t)a.rows * nc * 2 <= 3ull * a.sm_count && a.vocab / (nc * 2) >= 32000) nc *= 2;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim = {nc, 1, 1};

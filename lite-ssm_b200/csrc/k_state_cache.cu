@@ -99,7 +99,7 @@ __device__ __forceinline__ void store_codes4(Code* to, const float (&v)[4], cons
 // is taken from the end, so one very large dt costs the tokens after it no digits.
 __device__ __forceinline__ void window_weights(float a, float dt, uint32_t lane, uint32_t count, float* w, float* alpha) {
     if (lane >= count) dt = 0.0f;
-    float s = a * dt;
+    float s = lane < count ? a * dt : 0.0f;   // a may be -inf
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const float t = __shfl_down_sync(0xffffffffu, s, o);

@@ -38,6 +38,7 @@ A = 0x10000  # an aligned address nothing dereferences: the calls are refused
     ((A, A, A, A, A, A, A, lssm.LogprobsDims(2, 10, 11, 0, 0)), "top_k"),
     ((A, A, A, A, A, A, A, lssm.LogprobsDims(2, 10, 4, 0, 9)), "row_stride"),
     ((A, A, A, A, A, A, A, lssm.LogprobsDims(2, 10, 4, 0, 1 << 41)), "row_stride"),
+    ((A, A, A, A, A, A, A, lssm.LogprobsDims(1 << 20, 10, 4, 0, 1 << 40)), "row_stride"),
     ((A, A, A, A, A, A, A, lssm.LogprobsDims(2, 10, 0, 0, 0)), "top_ids"),
     ((A, A, A, A, A, None, A, lssm.LogprobsDims(2, 10, 4, 0, 0)), "top_ids"),
     ((A, A, A, A, A, A, None, lssm.LogprobsDims(2, 10, 4, 0, 0)), "top_ids"),
@@ -396,9 +397,9 @@ def test_logprobs_gradient_against_differences(ctx):
 
 
 @pytest.mark.gpu
-def test_logprobs_captured_and_replayed(ctx):
+@pytest.mark.parametrize("V,k,rows", [(5003, 8, 3), (150001, 20, 2)])   # a CTA a row; a cluster a row
+def test_logprobs_captured_and_replayed(ctx, V, k, rows):
     """The call in a captured batch, replayed on new logits in the same buffers."""
-    V, k, rows = 5003, 8, 3
     rng = np.random.default_rng(2)
     c = lssm.Ctx(0)
     c.set_graph_batching(True)
@@ -418,3 +419,46 @@ def test_logprobs_captured_and_replayed(ctx):
         got["ids"], got["top"] = bi.download(np.uint32, rows * k).reshape(rows, k), bv.download(np.float32, rows * k).reshape(rows, k)
         check_rows(got, x64, t, V, k)
     c.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("V,k,rows", [(64003, 32, 3), (128000, 7, 2), (256001, 20, 5)])
+def test_logprobs_in_clusters(ctx, dt, V, k, rows):
+    """Rows split over 2, 4 and 8 CTAs: equal entries, masks and the largest entry in every slice."""
+    rng = np.random.default_rng(V)
+    x = np.round(logits(rng, rows, V), 1)          # many equal entries
+    x[0, V // 2:] = -np.inf                        # a slice, or half of them, with nothing left
+    x[1] = np.where(rng.random(V) < 0.9999, -np.inf, x[1])
+    x[rows - 1, [0, V // 3, V - 1]] = 30.0
+    arr, x64 = encode(x, dt)
+    t = np.array([V - 1, 5, V // 3, 0, NONE][:rows], np.uint32)
+    check_rows(call(ctx, arr, t, V, k, dt), x64, t, V, k)
+
+
+@pytest.mark.gpu
+def test_logprobs_two_contexts_on_streams_of_their_own(ctx):
+    """Calls of two contexts in flight together do not meet: nothing is shared between them."""
+    rng = np.random.default_rng(4)
+    V, k, rows = 40009, 9, 40
+    cs = [lssm.Ctx(0), lssm.Ctx(0)]
+    made = []
+    for c in cs:
+        arr, x64 = encode(logits(rng, rows, V), lssm.DT_F16)
+        t = rng.integers(0, V, rows).astype(np.uint32)
+        bufs = [lssm.DeviceBuffer.from_array(c, arr), lssm.DeviceBuffer.from_array(c, t)]
+        out = [lssm.DeviceBuffer(c, rows * 4) for _ in range(3)] + [lssm.DeviceBuffer(c, rows * k * 4) for _ in range(2)]
+        made.append((x64, t, bufs, out))
+    for c in cs:
+        c.begin_batch()
+    for _ in range(20):
+        for c, (x64, t, bufs, out) in zip(cs, made):
+            lssm.Ops(c).logprobs(*bufs, *out, lssm.LogprobsDims(rows, V, k, lssm.DT_F16, 0))
+    for c in cs:
+        c.commit_and_wait()
+    for x64, t, bufs, out in made:
+        got = dict(zip(("logp", "entropy", "lse"), (q.download(np.float32, rows) for q in out)))
+        got["ids"], got["top"] = out[3].download(np.uint32, rows * k).reshape(rows, k), out[4].download(np.float32, rows * k).reshape(rows, k)
+        check_rows(got, x64, t, V, k)
+    for c in cs:
+        c.close()

@@ -93,6 +93,10 @@ def test_load_and_store_arguments_refused():
     refuse(load_args(d, c), "null context")
     refuse(step_args(d, c), "null context")
     refuse(step_args(dims(has_D=0), c, D=None), "null context")   # D is not looked at without has_D
+    nothing = cache_ptrs(**{n: None for n in ("codes", "scales", "win_x", "win_B", "win_dt", "fill")})
+    for kw in (dict(batch=0), dict(H=0), dict(P=0), dict(N=0)):   # an empty cache has no arrays
+        for call in (store_args(dims(**kw), nothing, None), load_args(dims(**kw), nothing, None, None), step_args(dims(**kw), nothing)):
+            refuse(call, "null context")
 
 
 def test_bytes():
@@ -423,3 +427,59 @@ def test_captured_step_replays_through_a_fold(ctx, bits):
         if (c.fill() == 0).all():
             c.pull()
     cc.close()
+
+
+@pytest.mark.gpu
+def test_empty_calls_do_nothing(ctx):
+    none = lssm.StateCache.wrap(None, None, None, None, None, None)
+    ops = lssm.Ops(ctx)
+    for kw in (dict(batch=0), dict(H=0), dict(P=0), dict(N=0)):
+        d = dims(**kw)
+        ops.state_cache_store(None, none, d)
+        ops.state_cache_load(none, None, None, lssm.DT_F32, d)
+        ops.ssd_step_cached(None, None, None, None, None, None, None, none, None, d)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("which", ["codes", "win_x", "win_B", "x", "B", "C", "state"])
+def test_arrays_off_by_an_element(ctx, which, bits):
+    """Arrays aligned to their element only: the common shape leaves its 16-byte path."""
+    rng = np.random.default_rng(21)
+    d = dims(2, 4, 64, 128, 1, 3, bits)
+    c = Cache(ctx, d, rng)
+    es = bits // 8 if which == "codes" else 4 if which == "state" else 2
+    keep = []
+
+    def shifted(a):
+        raw = np.ascontiguousarray(a).view(np.uint8).reshape(-1)
+        b = lssm.DeviceBuffer.from_array(ctx, np.concatenate([np.zeros(es, np.uint8), raw, np.zeros(64, np.uint8)]))
+        keep.append(b)
+        return lssm.DeviceView(ctx, b.ptr.value + es)
+
+    names = ("codes", "scales", "win_x", "win_B", "win_dt", "fill")
+    ptrs = dict(zip(names, (b.ptr.value for b in c.cache.buffers)))
+    if which in ptrs:
+        b = c.cache.buffers[names.index(which)]
+        ptrs[which] = shifted(b.download(np.uint8, b.nbytes)).ptr.value
+    cache = lssm.StateCache.wrap(*(ptrs[n] for n in names))
+    up = lambda a, n: shifted(a) if n == which else lssm.DeviceBuffer.from_array(ctx, a)  # noqa: E731
+    for i in range(5):
+        tok = c.token(rng)
+        y = lssm.DeviceBuffer(ctx, c.B * c.H * c.P * 2)
+        c.ops.ssd_step_cached(*(up(a, n) for a, n in zip(tok, ("x", "B", "C", "dt"))), c.dbias, c.dA, c.dD, cache, y, d)
+        want, off_y = c.advance(tok)
+        got = y.download(np.float16, c.B * c.H * c.P).reshape(c.B, c.H, c.P).astype(np.float64)
+        assert (np.abs(got - want) <= 2.0 ** -11 * np.abs(want) + off_y + 2.0 ** -25).all()
+        out = shifted(np.zeros(c.S.shape, np.float32)) if which == "state" else lssm.DeviceBuffer(ctx, c.S.size * 4)
+        c.ops.state_cache_load(cache, c.dA, out, lssm.DT_F32, d)
+        host = np.empty(c.S.size, np.float32)
+        lssm.check(lssm.lib().lssm_download(ctx.h, host.ctypes.data_as(lssm.P), out.ptr, 0, host.nbytes))
+        held = host.astype(np.float64).reshape(c.S.shape)
+        if (i + 1) % 3 == 0:   # folded: within half a step of the state, and exactly what goes on from here
+            Q = 127 if bits == 8 else 32767
+            lim = np.abs(c.S).max(-1, keepdims=True) / Q * (0.5 + 1e-4) + 2 * c.tol().max(-1, keepdims=True)
+            assert (np.abs(held - c.S) <= lim).all()
+            c.S, c.size, c.err = held, np.abs(held), np.zeros_like(held)
+        else:
+            assert (np.abs(held - c.S) <= c.tol() + U * np.abs(c.S)).all()
