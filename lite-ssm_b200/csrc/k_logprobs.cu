@@ -21,6 +21,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32, LP_TOPS = 32 / LP_WARPS;
+constexpr int LP_AHEAD = 2048;       // 16-byte chunks of a later row that a CTA asks L2 for
 constexpr int LP_GROUP = 4;          // 16-byte loads that a thread has on their way while it works on as many
 constexpr int LP_CTAS = 4;           // CTAs an SM holds
 constexpr int LP_CAND = 1024;        // candidates for the top entries that a CTA holds
@@ -111,14 +112,6 @@ struct Row {
             for (int i = 0; i < VEC; ++i) t[i] = e + i >= 0 && e + i < (int64_t)V ? x[e + i] : lowest();
             memcpy(&r, t, 16);
         }
-        return r;
-    }
-    static __device__ __forceinline__ uint4 nothing() {
-        T t[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) t[i] = lowest();
-        uint4 r;
-        memcpy(&r, t, 16);
         return r;
     }
 };
@@ -500,6 +493,16 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) k_logprobs(LogprobsArgs a
         if (!groups) break;
         if (--groups) load(w);
         work(next);
+    }
+    // HBM has nothing to do for this CTA from here on: the beginning of the row one full GPU of CTAs ahead goes to L2
+    // (2048 x 50288 fp16, 20 alternatives: 50.4 us without, 49.2 with 16 KB, 47.1 with 32 or 64, 51.1 with 128).
+    const uint64_t later = (uint64_t)r + (uint32_t)(a.sm_count * LP_CTAS);
+    if (nc == 1 && tid == 0 && later < a.rows) {
+        const Row<T> next_row(a.logits, later * a.row_stride, a.vocab);
+        const uint32_t n = min(next_row.outer() - next_row.inner(), (uint32_t)LP_AHEAD);
+        if (next_row.outer() > next_row.inner())
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
+                         ::"l"(__cvta_generic_to_global(next_row.base() + next_row.inner())), "r"(n * 16) : "memory");
     }
     float xt = 0.0f;
     if (target < a.vocab) xt = load_one(row.x + target);

@@ -437,6 +437,21 @@ def test_logprobs_in_clusters(ctx, dt, V, k, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("V,pad,off,k", [(1, 0, 0, 1), (5, 2, 3, 2), (1501, 6, 1, 4), (12007, 1, 0, 3)])
+def test_logprobs_more_rows_than_ctas(ctx, dt, V, pad, off, k):
+    """Rows of later waves, whose beginnings earlier ones ask for: the last rows end with the array."""
+    rows = 1400
+    rng = np.random.default_rng(V)
+    few = np.pad(logits(rng, 35, V), ((0, 0), (0, pad)))
+    full = np.concatenate([np.zeros(off), np.tile(few, (rows // 35, 1)).ravel()])[:off + rows * (V + pad) - pad]
+    arr, _ = encode(full, dt)
+    _, x64 = encode(few[:, :V], dt)
+    t = rng.integers(0, V, rows).astype(np.uint32)
+    check_rows(call(ctx, arr, t, V, k, dt, stride=V + pad, off=off), np.tile(x64, (rows // 35, 1)), t, V, k)
+
+
+@pytest.mark.gpu
 def test_logprobs_two_contexts_on_streams_of_their_own(ctx):
     """Calls of two contexts in flight together do not meet: nothing is shared between them."""
     rng = np.random.default_rng(4)
