@@ -437,6 +437,23 @@ __device__ __forceinline__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t
 }
 
 // One CTA, or a cluster of nc over slices of the vocabulary, per row; one pass over the logits.
+//
+// The pass: a thread keeps s and u against its own lagging reference, and its largest entry; the threads' sums meet
+// against the row's maximum m with e^(x - ref) = e^(x - m) e^(m - ref), where u moves by s (ref - m) too. The row is
+// read once from HBM; cta_top's second look at a few chunks finds them in L2. Nothing between the kernel's phases
+// goes through memory, so there is no workspace and no second launch.
+//
+// Why so: 256 threads x 2 groups of 4 x 16 bytes on their way, 4 CTAs an SM, put 128 KB of loads on an SM; the
+// registers (64 a thread) allow no more. fp16 entries are worked on two a time (f32x2), with one ex2 each.
+// What bounds it, at 2048 x 50288 fp16 with 20 alternatives: 47.1 us = 4.4 TB/s, 67 % of a copy's rate. Without
+// alternatives 41 us, as a pass that only reads in this loop takes 37: the selection after a CTA's pass (barriers and
+// second reads, a third of its cycles) leaves HBM idle where the other CTAs of the SM are in it too, and 2048 rows are
+// 3.5 waves. 333 x 32001 fp32, 8 alternatives: 14.4 us; 64 x 256000 fp16, 5 of them: 14.4 us; one row of 50288: 8.2 us,
+// latency of a launch, of reads one after the other and of barriers.
+// Measured and not kept: a ring of bulk or 16-byte asynchronous copies in shared memory (54-56 us: the second trip
+// through shared memory costs issue slots), 128 threads a CTA (56), CTAs that start at different places (49 where 50 was),
+// CTAs that walk over rows with the next row's first chunks copied ahead (107: spills), the last wave's rows split over
+// clusters (51).
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) k_logprobs(LogprobsArgs a, uint32_t nc) {
     __shared__ LpShared sh;
@@ -640,6 +657,9 @@ __device__ __forceinline__ void store_chunk(G* p, const float (&v)[n]) {
 // logits); all of them are loaded before the first is worked on. Where the chunks' places in the output are not
 // aligned for wide stores, a warp exchanges its 32 chunks through shared memory, so that a store instruction
 // writes 32 neighbours.
+// Bound by HBM: 2048 x 50288 fp16 to fp16 69.6 us = 5.9 TB/s, 90 % of a copy's rate (the same with a third fewer
+// instructions, in pairs of entries: not kept); 257 x 32001 bf16 to fp32 with the entropy's term, rows at odd addresses,
+// 12.6 us = 3.9 TB/s (35 us with stores of one element, before the exchange), where a launch's ends weigh more.
 constexpr int GRAD_CHUNKS = 4;
 template <typename T, typename G, bool ENTROPY>
 __global__ void __launch_bounds__(LP_THREADS) k_logprobs_grad(LogprobsGradArgs a, uint32_t parts) {

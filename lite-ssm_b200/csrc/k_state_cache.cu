@@ -117,6 +117,8 @@ constexpr int SC_THREADS = 256;
 // row, so neighbours are read and written together whatever N and the arrays' alignment are.
 // A step: S_q C of the rows by warps, C . B_j of the window's tokens by warps, then y by a thread a row.
 // A fold or a load: a warp keeps 32 elements of every B_j in registers (KB * 16 of them) and walks down the rows.
+// Only for P or N above 256, which no known model has: it is right for every shape, and issue bounds it (the products
+// are on the CUDA cores). With the shapes above that k_state_tc takes it took twice that kernel's time.
 constexpr uint32_t ANY_ROWS = 128, ANY_ILP = 8;   // rows at a time; of them, rows a warp has on their way
 template <typename Code, int MODE, int KB>
 __global__ void __launch_bounds__(SC_THREADS, KB == 1 ? 3 : 2) k_state_any(StateCacheArgs a) {
@@ -386,9 +388,31 @@ struct TcShared {
 
 __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
+// A step or a load on the tensor cores. A CTA takes the codes of one to TC_HEADS heads of a group: they share the
+// window's B, C and C . B_j. MODE 0: a step, which folds where it fills the window; MODE 1: a load.
 // KB: blocks of 16 window tokens (W <= 16 * KB). Grid: blocks of heads, groups, sequences.
 // PAD: any N up to the template's and any P, alignment and stride: one head a CTA, read and written element by element,
 // with zeros behind its rows and columns.
+//
+// y = alpha scale (code . C) + sum_j w_j (C . B_j) x_j + D x: the codes are the A operand as they are, since whole
+// numbers up to 2048 are exact in f16 (16 bits: two bytes, 256 hi + lo), and C is an f16 input: the product has no
+// rounding but its fp32 sums'. Bytes become f16 by one byte permutation into 0x64.. and one subtraction, so that no
+// conversion runs. A fold or load adds sum_j (w_j x_j) B_j^T, the product of two 16 x W operands: w_j x_j, an fp32
+// product, goes in as two f16 terms (22 bits), scaled by a power of two so that neither leaves f16's range.
+// Codes wait in shared memory in an order that lets a lane take 16 bytes of a row without two lanes on one bank.
+//
+// What bounds it, at 64 sequences x 80 heads of 64 x 128, 8 bits, W 16: 17.2 us without a fold (42 MB of codes, 47 MB
+// in all; 2.7 TB/s, 41 % of a copy's rate). 1280 CTAs of about 6 us are 2.2 waves of 4 CTAs an SM, each a chain of
+// reads, three barriers and products: latency and issue, not HBM. With one sequence in 16 folding at each step, as
+// sequences that began at different times do, 26.4 us; with all of them folding 57 us, once in 16 steps. The fp32 step
+// (ssd_step_batched) takes 51 us each time. 16 bits: 25.0 us. One sequence of 24 heads: 4.1 us, a launch's latency.
+// A load of the same 64 sequences takes 32.6 us to fp16 (126 MB, 3.9 TB/s; the products' and the stores' issue) and
+// 39 us to fp32 (210 MB, 5.4 TB/s; HBM). 16 sequences x 64 heads of 75 x 203, 8 bits, padded: 28 us a step (55 on the
+// CUDA cores).
+// Measured and not kept: a persistent CTA with the next heads' codes on their way (24.8-30 us against 23.8 at the time:
+// registers for two of everything leave 2 CTAs an SM), codes in two parts that are waited for one after the other
+// (18.6 against 17.2), all W rows of the window read without waiting for `fill` (19.3; one sequence 5.0 against 4.1),
+// 3 or 5 CTAs an SM, CTAs of half the size (19.0), odd N's codes through an aligned copy in shared memory.
 template <typename Code, int MODE, int KB, int N, bool PAD>
 __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_state_tc(StateCacheArgs a, uint32_t heads, uint32_t per_group) {
     constexpr float Q = sizeof(Code) == 1 ? 127.0f : 32767.0f;
@@ -766,6 +790,7 @@ cudaError_t launch_cached(const StateCacheArgs& a, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+// N above 256: a warp a row, read twice (the second time from L2).
 template <typename Code>
 __global__ void __launch_bounds__(SC_THREADS) k_state_store(StateCacheArgs a) {
     constexpr float Q = sizeof(Code) == 1 ? 127.0f : 32767.0f;
@@ -787,6 +812,8 @@ __global__ void __launch_bounds__(SC_THREADS) k_state_store(StateCacheArgs a) {
     }
 }
 
+// Rounding a state into codes: one read, one write, bound by HBM: 64 sequences x 80 heads of 64 x 128, 8 bits, 36 us for
+// 210 MB = 5.8 TB/s, 88 % of a copy's rate.
 // N up to 256: a warp takes ROWS rows, a lane PER elements of each in registers: VEC neighbours at a time (VEC 4: N a
 // multiple of 4 and the arrays aligned for it), runs of 32 * VEC. Lane r works out row r's scale. The largest magnitude
 // is found on the bits of |v|, which order as the values do, with NaN above infinity.
