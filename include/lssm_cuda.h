@@ -325,7 +325,7 @@ lssm_status lssm_state_cache_load(lssm_ctx* ctx, lssm_state_cache cache, const v
 /* lssm_ssd_step_batched over the cache: one decode token of dims.batch sequences, fp16 x (batch, H*P),
  * B / C (batch, G*N), dt_raw (batch, H), dt_bias / A_log / D (H), fp16 y (batch, H*P). A_log must be
  * the same at every step of a window. The call is the same whatever the windows hold, so a captured
- * step may be replayed. */
+ * step may be replayed. y and the cache must not overlap the inputs or one another. */
 lssm_status lssm_ssd_step_cached(lssm_ctx* ctx, const void* x, const void* B, const void* C, const void* dt_raw,
                                  const void* dt_bias, const void* A_log, const void* D_skip, lssm_state_cache cache,
                                  void* y, lssm_state_cache_dims dims);

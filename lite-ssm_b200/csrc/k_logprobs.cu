@@ -451,9 +451,9 @@ __device__ __forceinline__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t
 // 3.5 waves. 333 x 32001 fp32, 8 alternatives: 14.4 us; 64 x 256000 fp16, 5 of them: 14.4 us; one row of 50288: 8.2 us,
 // latency of a launch, of reads one after the other and of barriers.
 // Measured and not kept: a ring of bulk or 16-byte asynchronous copies in shared memory (54-56 us: the second trip
-// through shared memory costs issue slots), 128 threads a CTA (56), CTAs that start at different places (49 where 50 was),
-// CTAs that walk over rows with the next row's first chunks copied ahead (107: spills), the last wave's rows split over
-// clusters (51).
+// through shared memory costs issue slots), 128 threads a CTA (56), CTAs that start at different places (49 where 50
+// was), CTAs that walk over rows with the next row's first chunks copied ahead (107: spills), the last wave's rows
+// split over clusters (51).
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) k_logprobs(LogprobsArgs a, uint32_t nc) {
     __shared__ LpShared sh;
