@@ -370,7 +370,7 @@ struct Pow2 {
 template <typename Code, int KB, int N>
 struct TcShared {
     static constexpr uint32_t ROW = N * sizeof(Code), PIECES = ROW / 16;
-    static constexpr uint32_t B_PITCH = N * 2 + 16, PAIR_PITCH = N + 16;   // bytes; words
+    static constexpr uint32_t B_PITCH = N * 2 + 16, PAIR_PITCH = N + 8;   // bytes; words
     uint32_t x_pitch, x, B, C, dot, pairs, total;   // bytes from the start; codes are first
     __host__ __device__ TcShared(uint32_t rows) {   // rows: heads * P
         x_pitch = rows * 2 + 16;
@@ -406,15 +406,16 @@ __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_c
 // reads, three barriers and products: latency and issue, not HBM. With one sequence in 16 folding at each step, as
 // sequences that began at different times do, 26.4 us; with all of them folding 57 us, once in 16 steps. The fp32 step
 // (ssd_step_batched) takes 51 us each time. 16 bits: 25.0 us. One sequence of 24 heads: 4.1 us, a launch's latency.
-// A load of the same 64 sequences takes 32.6 us to fp16 (126 MB, 3.9 TB/s; the products' and the stores' issue) and
-// 39 us to fp32 (210 MB, 5.4 TB/s; HBM). 16 sequences x 64 heads of 75 x 203, 8 bits, padded: 28 us a step (55 on the
+// A load of the same 64 sequences takes 29.5 us to fp16 (126 MB, 4.3 TB/s; shared memory's and the products' latency:
+// 32.6 with 8-byte stores and two-way conflicts on the pairs) and 38.6 us to fp32 (210 MB, 5.4 TB/s; HBM).
+// 16 sequences x 64 heads of 75 x 203, 8 bits, padded: 28 us a step (55 on the
 // CUDA cores).
 // Measured and not kept: a persistent CTA with the next heads' codes on their way (24.8-30 us against 23.8 at the time:
 // registers for two of everything leave 2 CTAs an SM), codes in two parts that are waited for one after the other
 // (18.6 against 17.2), all W rows of the window read without waiting for `fill` (19.3; one sequence 5.0 against 4.1),
 // 3 or 5 CTAs an SM, CTAs of half the size (19.0), odd N's codes through an aligned copy in shared memory.
 template <typename Code, int MODE, int KB, int N, bool PAD>
-__global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_state_tc(StateCacheArgs a, uint32_t heads, uint32_t per_group) {
+__global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateCacheArgs a, uint32_t heads, uint32_t per_group) {
     constexpr float Q = sizeof(Code) == 1 ? 127.0f : 32767.0f;
     using Sh = TcShared<Code, KB, N>;
     extern __shared__ __align__(128) uint8_t sm[];
@@ -681,6 +682,33 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
             const uint64_t o0 = ((uint64_t)bh0 * a.P + row) * n_real + 4 * t;
             // padded rows and columns are left out; without them, stores of four where the state's rows allow it
             const bool wide = !PAD || (a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.state) & 15) == 0);
+            auto pack16 = [&](const float (&v)[4]) {
+                if (a.state_dtype == LSSM_DT_F16)
+                    return make_uint2(h2_bits(__floats2half2_rn(v[0], v[1])), h2_bits(__floats2half2_rn(v[2], v[3])));
+                const __nv_bfloat162 m0 = __floats2bfloat162_rn(v[0], v[1]), m1 = __floats2bfloat162_rn(v[2], v[3]);
+                uint2 w;
+                memcpy(&w.x, &m0, 4);
+                memcpy(&w.y, &m1, 4);
+                return w;
+            };
+            if (!PAD && a.state_dtype != LSSM_DT_F32) {
+                // two words at a time: lanes t and t ^ 1 exchange, so that each stores 8 neighbours, the even one of q
+                const bool odd = t & 1;
+                uint16_t* out = static_cast<uint16_t*>(a.state) + o0 + (odd ? 12 : 0);
+#pragma unroll
+                for (int q = 0; q < N / 16; q += 2) {
+                    float s0[2][4], s1[2][4];
+                    word(q, s0);
+                    word(q + 1, s1);
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const uint2 w0 = pack16(s0[r]), w1 = pack16(s1[r]);
+                        const uint32_t x = __shfl_xor_sync(0xffffffffu, odd ? w0.x : w1.x, 1), y = __shfl_xor_sync(0xffffffffu, odd ? w0.y : w1.y, 1);
+                        __stcs(reinterpret_cast<uint4*>(out + 8 * n_real * r + 16 * q),
+                               odd ? make_uint4(x, y, w1.x, w1.y) : make_uint4(w0.x, w0.y, x, y));
+                    }
+                }
+            } else
 #pragma unroll
             for (int q = 0; q < N / 16; ++q) {
                 float s[2][4];
@@ -695,17 +723,8 @@ __global__ void __launch_bounds__(TC_THREADS, MODE == 0 && KB == 1 ? 4 : 3) k_st
                             if (16 * q + 4 * t + i < n_real) store_any(a.state, o + i, a.state_dtype, s[r][i]);
                     } else if (a.state_dtype == LSSM_DT_F32)
                         __stcs(reinterpret_cast<float4*>(static_cast<float*>(a.state) + o), make_float4(s[r][0], s[r][1], s[r][2], s[r][3]));
-                    else {
-                        uint2 w;
-                        if (a.state_dtype == LSSM_DT_F16)
-                            w = make_uint2(h2_bits(__floats2half2_rn(s[r][0], s[r][1])), h2_bits(__floats2half2_rn(s[r][2], s[r][3])));
-                        else {
-                            const __nv_bfloat162 m0 = __floats2bfloat162_rn(s[r][0], s[r][1]), m1 = __floats2bfloat162_rn(s[r][2], s[r][3]);
-                            memcpy(&w.x, &m0, 4);
-                            memcpy(&w.y, &m1, 4);
-                        }
-                        __stcs(reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.state) + o), w);
-                    }
+                    else
+                        __stcs(reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.state) + o), pack16(s[r]));
                 }
             }
         } else {
