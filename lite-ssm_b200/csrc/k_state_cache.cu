@@ -408,12 +408,12 @@ __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_c
 // (ssd_step_batched) takes 51 us each time. 16 bits: 25.0 us. One sequence of 24 heads: 4.1 us, a launch's latency.
 // A load of the same 64 sequences takes 29.5 us to fp16 (126 MB, 4.3 TB/s; shared memory's and the products' latency:
 // 32.6 with 8-byte stores and two-way conflicts on the pairs) and 38.6 us to fp32 (210 MB, 5.4 TB/s; HBM).
-// 16 sequences x 64 heads of 75 x 203, 8 bits, padded: 28 us a step (55 on the
-// CUDA cores).
+// 16 sequences x 64 heads of 75 x 203, 8 bits, padded: 28 us a step (55 on the CUDA cores).
 // Measured and not kept: a persistent CTA with the next heads' codes on their way (24.8-30 us against 23.8 at the time:
 // registers for two of everything leave 2 CTAs an SM), codes in two parts that are waited for one after the other
 // (18.6 against 17.2), all W rows of the window read without waiting for `fill` (19.3; one sequence 5.0 against 4.1),
-// 3 or 5 CTAs an SM, CTAs of half the size (19.0), odd N's codes through an aligned copy in shared memory.
+// 3 or 5 CTAs an SM, CTAs of half the size (19.0), odd N's codes through an aligned copy in shared memory; fp32 pairs
+// in one instruction (f32x2) for the fold and the load: 2 % less a step, 1 % more a load.
 template <typename Code, int MODE, int KB, int N, bool PAD>
 __global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateCacheArgs a, uint32_t heads, uint32_t per_group) {
     constexpr float Q = sizeof(Code) == 1 ? 127.0f : 32767.0f;
