@@ -277,14 +277,12 @@ __global__ void __launch_bounds__(SC_THREADS, KB == 1 ? 3 : 2) k_state_any(State
 //  N = 64, 128 or 256, P a multiple of 16: tensor-core kernel
 // ---------------------------------------------------------------------------
 // A CTA takes `heads` heads of one group and sequence; a warp 16 rows of a head's state at a time. With m16n8k16
-// (f16 in, f32 out), lane
-// (g, t) = (lane / 4, lane % 4), and an order of k that lets a lane load its codes as they lie:
+// (f16 in, f32 out), lane (g, t) = (lane / 4, lane % 4), and an order of k that lets a lane load its codes as they lie:
 //   S_q C       A = codes (exact in f16: 8 bits as they are, 16 bits as 256 * high + low), B = C in every column
 //   C . B_j     A = the window's B rows, B = C in every column (one warp; 16 tokens an instruction)
 //   sum_j w_j x_j B_j^T (fold, load)   A = w_j x_j[p] as two f16 terms (22 bits), scaled by a power of two that puts
 //               the largest at 2^14, B = the window's B; a lane gets the elements whose codes it holds.
-// A code is converted, multiplied and added in about one instruction for 30 elements, so the step is bound by the
-// codes' bytes and the latency of a short CTA.
+// A code is converted, multiplied and added in about one instruction for 30 elements.
 constexpr int TC_THREADS = 256, TC_WARPS = TC_THREADS / 32, TC_HEADS = 4;
 constexpr uint32_t TC_BYTES = 32 * 1024;   // of codes a CTA holds (one head may have more)
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
