@@ -284,6 +284,7 @@ __global__ void __launch_bounds__(SC_THREADS, KB == 1 ? 3 : 2) k_state_any(State
 //               the largest at 2^14, B = the window's B; a lane gets the elements whose codes it holds.
 // A code is converted, multiplied and added in about one instruction for 30 elements.
 constexpr int TC_THREADS = 256, TC_WARPS = TC_THREADS / 32, TC_HEADS = 4;
+constexpr uint32_t STAGE_PITCH = 48;        // words a row of a load's staged stores: two rows' lanes share no bank
 constexpr uint32_t TC_BYTES = 32 * 1024;   // of codes a CTA holds (one head may have more)
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -385,6 +386,10 @@ struct TcShared {
 };
 
 __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+
+// A padded load: four neighbours of the state in one store; if not, its 16-bit states through shared memory.
+__host__ __device__ __forceinline__ bool wide_rows(const StateCacheArgs& a) { return a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.state) & 15) == 0; }
+__host__ __device__ __forceinline__ bool staged_load(const StateCacheArgs& a) { return !wide_rows(a) && a.state_dtype != LSSM_DT_F32; }
 
 // A step or a load on the tensor cores. A CTA takes the codes of one to TC_HEADS heads of a group: they share the
 // window's B, C and C . B_j. MODE 0: a step, which folds where it fills the window; MODE 1: a load.
@@ -679,7 +684,7 @@ __global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateC
         if constexpr (MODE == 1) {
             const uint64_t o0 = ((uint64_t)bh0 * a.P + row) * n_real + 4 * t;
             // padded rows and columns are left out; without them, stores of four where the state's rows allow it
-            const bool wide = !PAD || (a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.state) & 15) == 0);
+            const bool wide = !PAD || wide_rows(a);
             auto pack16 = [&](const float (&v)[4]) {
                 if (a.state_dtype == LSSM_DT_F16)
                     return make_uint2(h2_bits(__floats2half2_rn(v[0], v[1])), h2_bits(__floats2half2_rn(v[2], v[3])));
@@ -705,6 +710,28 @@ __global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateC
                         __stcs(reinterpret_cast<uint4*>(out + 8 * n_real * r + 16 * q),
                                odd ? make_uint4(x, y, w1.x, w1.y) : make_uint4(w0.x, w0.y, x, y));
                     }
+                }
+            } else if (PAD && staged_load(a)) {
+                // 16 rows x 32 columns at a time through shared memory, so that a store instruction writes 32 neighbours
+                // (16 x 64 heads of 75 x 203, 8 bits, to fp16: 59 -> 43 us; to fp32, whose stores of one element fill
+                // more of a line, it costs 5 %)
+                float(*stage)[STAGE_PITCH] = reinterpret_cast<float(*)[STAGE_PITCH]>(sm + sh.total) + 16 * wid;
+                const uint64_t t0 = ((uint64_t)bh0 * a.P + tile * 16) * n_real;
+                for (int q = 0; q < N / 16 && 16u * q < n_real; q += 2) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float s[2][4];
+                        word(q + k, s);
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+                            *reinterpret_cast<float4*>(&stage[g + 8 * r][16 * k + 4 * t]) = make_float4(s[r][0], s[r][1], s[r][2], s[r][3]);
+                    }
+                    __syncwarp();
+                    const uint32_t e = 16 * q + lane;
+#pragma unroll
+                    for (uint32_t r = 0; r < 16; ++r)
+                        if (tile * 16 + r < real && e < n_real) store_any(a.state, t0 + r * n_real + e, a.state_dtype, stage[r][lane]);
+                    __syncwarp();
                 }
             } else
 #pragma unroll
@@ -773,7 +800,8 @@ cudaError_t launch_tc(const StateCacheArgs& a, cudaStream_t s) {
     uint32_t heads = PAD ? 1 : TC_HEADS;
     while (heads > 1 && (heads * a.P > TC_THREADS || heads * a.P * N * sizeof(Code) > TC_BYTES ||
                          (uint64_t)a.batch * a.G * ((per_group + heads - 1) / heads) < 2ull * 148)) heads /= 2;
-    const uint32_t bytes = TcShared<Code, KB, N>(PAD ? (a.P + 15) / 16 * 16 : heads * a.P).total;
+    const uint32_t bytes = TcShared<Code, KB, N>(PAD ? (a.P + 15) / 16 * 16 : heads * a.P).total +
+                           (PAD && MODE == 1 && staged_load(a) ? TC_WARPS * 16 * STAGE_PITCH * 4 : 0);
     const auto kernel = k_state_tc<Code, MODE, KB, N, PAD>;
     if (bytes > 36 * 1024) {   // with the static part, more than 48 KB
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);

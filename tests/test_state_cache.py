@@ -315,17 +315,22 @@ def test_store_many_random_rows_exact(ctx):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shape", [(2, 4, 64, 128, 1, 16), (1, 2, 7, 19, 2, 5)])
+@pytest.mark.parametrize("shape", [(2, 4, 64, 128, 1, 16), (1, 2, 7, 19, 2, 5), (1, 2, 255, 255, 1, 20), (2, 3, 75, 203, 1, 16),
+                                   (1, 1, 256, 256, 1, 32), (2, 4, 48, 64, 2, 7), (1, 2, 33, 300, 1, 4), (3, 2, 40, 100, 1, 9)])
 @pytest.mark.parametrize("dt,half", [(lssm.DT_F16, 2.0 ** -11), (lssm.DT_BF16, 2.0 ** -8), (lssm.DT_F32, U)])
 def test_load_types(ctx, shape, dt, half):
     rng = np.random.default_rng(6)
     for bits in (8, 16):
         c = Cache(ctx, dims(*shape, bits), rng)
+        tokens = 0
         for n in (0, 1, 3):
             for _ in range(n):
                 tok = c.token(rng)
                 c.step(tok)
                 c.advance(tok)
+                tokens += 1
+                if tokens == shape[5]:   # folded: the state is what the codes hold (a window of 4 fills here)
+                    c.pull()
             before = [b.download(np.uint8, b.nbytes) for b in c.cache.buffers]
             got = c.load(dt)
             assert (np.abs(got - c.S) <= half * np.abs(c.S) + c.tol() * (1 + half) + 2.0 ** -25).all()
@@ -438,6 +443,26 @@ def test_empty_calls_do_nothing(ctx):
         ops.state_cache_store(None, none, d)
         ops.state_cache_load(none, None, None, lssm.DT_F32, d)
         ops.ssd_step_cached(None, None, None, None, None, None, None, none, None, d)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2, 3, 64, 128, 1, 4), (1, 3, 75, 203, 1, 4), (2, 2, 17, 50, 1, 4)])
+@pytest.mark.parametrize("off", [0, 1, 3])
+def test_load_to_16_bits_writes_nothing_else(ctx, shape, off):
+    """A 16-bit state that begins at any element, with neighbours on both sides that stay as they are."""
+    rng = np.random.default_rng(off)
+    c = Cache(ctx, dims(*shape, 8), rng)
+    tok = c.token(rng)
+    c.step(tok)
+    c.advance(tok)
+    n = c.S.size
+    buf = lssm.DeviceBuffer.from_array(ctx, np.full(n + off + 40, 7.5, np.float16))
+    c.ops.state_cache_load(c.cache, c.dA, lssm.DeviceView(ctx, buf.ptr.value + 2 * off), lssm.DT_F16, c.d)
+    got = buf.download(np.float16, n + off + 40)
+    assert (got[:off] == 7.5).all() and (got[off + n:] == 7.5).all()
+    held = got[off:off + n].reshape(c.S.shape).astype(np.float64)
+    half = 2.0 ** -11
+    assert (np.abs(held - c.S) <= half * np.abs(c.S) + c.tol() * (1 + half) + 2.0 ** -25).all()
 
 
 @pytest.mark.gpu
