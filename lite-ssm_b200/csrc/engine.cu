@@ -1039,6 +1039,7 @@ static lssm_status states_to_f32(lssm_session* s, cudaStream_t st) {
 }
 static lssm_status set_state_cache(lssm_session* s, uint32_t bits, uint32_t window) {
     if (bits == s->state_bits && window == s->state_window) return LSSM_OK;
+    if (s->ctx->batch_active) return fail(LSSM_ERR_STATE, "lssm_session_set_option: a batch is active");
     if (lssm_status r = states_to_f32(s, s->ctx->stream)) return r;
     CU(cudaStreamSynchronize(s->ctx->stream));
     if (s->graph) { cudaGraphExecDestroy(s->graph); s->graph = nullptr; }

@@ -167,6 +167,9 @@ def test_scoring_refusals(ctx):
     try:
         refused("batch is active", L.lssm_score(s.h, p, 4, 0, o, None, None, None))
         refused("batch is active", L.lssm_session_logprobs(s.h, p, 0, o, None, None, None))
+        for key, value in (("state_bits", 8), ("state_window", 4)):
+            with pytest.raises(lssm.LssmError, match="batch is active"):
+                s.set_option(key, value)
     finally:
         ctx.commit_and_wait()
     for key, bad in (("state_bits", 4), ("state_bits", 32), ("state_window", 0), ("state_window", 33)):
