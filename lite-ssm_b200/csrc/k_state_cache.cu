@@ -280,8 +280,8 @@ __global__ void __launch_bounds__(SC_THREADS, KB == 1 ? 3 : 2) k_state_any(State
 // (f16 in, f32 out), lane (g, t) = (lane / 4, lane % 4), and an order of k that lets a lane load its codes as they lie:
 //   S_q C       A = codes (exact in f16: 8 bits as they are, 16 bits as 256 * high + low), B = C in every column
 //   C . B_j     A = the window's B rows, B = C in every column (one warp; 16 tokens an instruction)
-//   sum_j w_j x_j B_j^T (fold, load)   A = w_j x_j[p] as two f16 terms (22 bits), scaled by a power of two that puts
-//               the largest at 2^14, B = the window's B; a lane gets the elements whose codes it holds.
+//   sum_j w_j x_j B_j^T (fold, load)   m16n8k8 in tf32: A = w_j x_j[p] as two terms of 11 bits, which have fp32's range, B =
+//               the window's B (exact: f16 has 11 bits too); a lane gets the elements whose codes it holds.
 // A code is converted, multiplied and added in about one instruction for 30 elements.
 constexpr int TC_THREADS = 256, TC_WARPS = TC_THREADS / 32, TC_HEADS = 4;
 constexpr uint32_t STAGE_PITCH = 48;        // words a row of a load's staged stores: two rows' lanes share no bank
@@ -291,12 +291,10 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// the same from zero
-__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                               uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+__device__ __forceinline__ void mma1688(float (&d)[4], const uint32_t (&a)[4], float b0, float b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { uint32_t u; memcpy(&u, &h, 4); return u; }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { __half2 h; memcpy(&h, &u, 4); return h; }
@@ -338,30 +336,12 @@ __device__ __forceinline__ void ldmatrix_t(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
-// Two f16 terms of (x0, x1): 22 bits together.
-__device__ __forceinline__ void split2(float x0, float x1, uint32_t* hi, uint32_t* lo) {
-    const __half2 h = __floats2half2_rn(x0, x1);
-    const float2 f = __half22float2(h);
-    *hi = h2_bits(h);
-    *lo = h2_bits(__floats2half2_rn(x0 - f.x, x1 - f.y));
+// Two tf32 terms of v: 22 bits together, whatever its size (the second is lost below 2^-115).
+__device__ __forceinline__ uint32_t tf32_bits(float v) { uint32_t u; asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(u) : "f"(v)); return u; }
+__device__ __forceinline__ void split2(float v, uint32_t* hi, uint32_t* lo) {
+    *hi = tf32_bits(v);
+    *lo = tf32_bits(v - __uint_as_float(*hi));
 }
-// A power of two that brings the largest of the warp's values to 2^14, and its inverse. Values that are not finite
-// set no scale.
-struct Pow2 {
-    float up, down;
-    template <int n>
-    __device__ __forceinline__ Pow2(const float (&v)[n]) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < n; ++i) {
-            const uint32_t bits = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-            if (bits < 0x7F800000u) top = max(top, bits);
-        }
-        const uint32_t eb = max(__reduce_max_sync(0xffffffffu, top) >> 23, 15u);
-        up = __uint_as_float(min(268u - eb, 254u) << 23);
-        down = __uint_as_float((eb - 14u) << 23);
-    }
-};
 
 // Shared memory of a CTA: the heads' codes (rows of N, their 16-byte pieces exchanged by row so that neither
 // 16-byte nor 4-byte reads of 8 rows meet in a bank), the window's x (a row a token) and B, C,
@@ -401,16 +381,19 @@ __host__ __device__ __forceinline__ bool staged_load(const StateCacheArgs& a) { 
 // numbers up to 2048 are exact in f16 (16 bits: two bytes, 256 hi + lo), and C is an f16 input: the product has no
 // rounding but its fp32 sums'. Bytes become f16 by one byte permutation into 0x64.. and one subtraction, so that no
 // conversion runs. A fold or load adds sum_j (w_j x_j) B_j^T, the product of two 16 x W operands: w_j x_j, an fp32
-// product, goes in as two f16 terms (22 bits), scaled by a power of two so that neither leaves f16's range.
+// product, goes in as two tf32 terms (22 bits). f16 terms would want a scale, and under any that rows or tokens share,
+// the small ones lose digits to the large ones: decays alone put 2^37 between a window's first token and its last. They take
+// half as many instructions and were faster at the 64 sequences below: a step with folds 26.2 us against 27.6, a load to fp16
+// 29.7 against 31.1 (with W 32 29.3 against 32.3 and 37.5 against 48.9).
 // Codes wait in shared memory in an order that lets a lane take 16 bytes of a row without two lanes on one bank.
 //
-// What bounds it, at 64 sequences x 80 heads of 64 x 128, 8 bits, W 16: 17.2 us without a fold (42 MB of codes, 47 MB
-// in all; 2.7 TB/s, 41 % of a copy's rate). 1280 CTAs of about 6 us are 2.2 waves of 4 CTAs an SM, each a chain of
+// What bounds it, at 64 sequences x 80 heads of 64 x 128, 8 bits, W 16: 17.0 us without a fold (42 MB of codes, 47 MB
+// in all; 2.8 TB/s, 42 % of a copy's rate). 1280 CTAs of about 6 us are 2.2 waves of 4 CTAs an SM, each a chain of
 // reads, three barriers and products: latency and issue, not HBM. With one sequence in 16 folding at each step, as
-// sequences that began at different times do, 26.4 us; with all of them folding 57 us, once in 16 steps. The fp32 step
+// sequences that began at different times do, 27.6 us; with all of them folding 60 us, once in 16 steps. The fp32 step
 // (ssd_step_batched) takes 51 us each time. 16 bits: 25.0 us. One sequence of 24 heads: 4.1 us, a launch's latency.
-// A load of the same 64 sequences takes 29.5 us to fp16 (126 MB, 4.3 TB/s; shared memory's and the products' latency:
-// 32.6 with 8-byte stores and two-way conflicts on the pairs) and 38.6 us to fp32 (210 MB, 5.4 TB/s; HBM).
+// A load of the same 64 sequences takes 31.1 us to fp16 (126 MB, 4.1 TB/s; shared memory's and the products' latency)
+// and 38.8 us to fp32 (210 MB, 5.4 TB/s; HBM).
 // 16 sequences x 64 heads of 75 x 203, 8 bits, padded: 28 us a step (55 on the CUDA cores).
 // Measured and not kept: a persistent CTA with the next heads' codes on their way (24.8-30 us against 23.8 at the time:
 // registers for two of everything leave 2 CTAs an SM), codes in two parts that are waited for one after the other
@@ -639,13 +622,12 @@ __global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateC
                 xw[8 * k + 2 * i + 1] = w.y * f.y;
             }
         }
-        // the window's part of the state: w_j x_j[p] in two f16 terms, scaled, times the window's B
-        const Pow2 p2(xw);
-        uint32_t ah[KB][4], al[KB][4];
+        // products of eight tokens: the first of a block of 16 has the lane's tokens 2t, 2t + 1, the second the other two
+        uint32_t ah[2 * KB][4], al[2 * KB][4];
 #pragma unroll
-        for (int k = 0; k < KB; ++k)
+        for (int k = 0; k < 2 * KB; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) split2(xw[8 * k + 2 * i] * p2.up, xw[8 * k + 2 * i + 1] * p2.up, &ah[k][i], &al[k][i]);
+            for (int i = 0; i < 4; ++i) split2(xw[4 * k + 2 * (i & 1) + (i >> 1)], &ah[k][i], &al[k][i]);
         // elements 16 q + 4 t .. + 3 of the state, rows g and g + 8. Their codes: piece q (8 bits; 16 bits: 2 q + t / 2),
         // exchanged, so the address for q differs from the one for 0 in the bits of q alone
         const uint32_t in_piece = 4 * t * sizeof(Code), at0 = row * Sh::ROW + (((in_piece >> 4) ^ sw) << 4) + (in_piece & 15);
@@ -659,26 +641,31 @@ __global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateC
 #pragma unroll
             for (int i = 0; i < 4; ++i) { s[0][i] = as[0] * cu[i]; s[1][i] = as[1] * cv[i]; }
             if (MODE == 1 && !count) return;
-            // column c of a product is element 16 q + 4 (c / 2) + c % 2 + 2 half: a lane gets what its codes are
-            float d[2][4];
+            // column c of a product is element 16 q + 4 (c / 2) + c % 2 + 2 half: a lane gets what its codes are. W <= 16
+            // sums onto the codes' part (a load to fp16: 33.0 -> 31.1 us); beyond that it would spill.
+            float d[2][4] = {};
+            if constexpr (KB == 1) {
 #pragma unroll
-            for (int k = 0; k < KB; ++k) {
-                const uint2 b0 = *reinterpret_cast<const uint2*>(pair0 + 8 * k * Sh::PAIR_PITCH + 16 * q);
-                const uint2 b1 = *reinterpret_cast<const uint2*>(pair0 + (8 * k + 4) * Sh::PAIR_PITCH + 16 * q);
-                if (k == 0) {
-                    mma16816_first(d[0], ah[k][0], ah[k][1], ah[k][2], ah[k][3], b0.x, b1.x);
-                    mma16816_first(d[1], ah[k][0], ah[k][1], ah[k][2], ah[k][3], b0.y, b1.y);
-                } else {
-                    mma16816(d[0], ah[k][0], ah[k][1], ah[k][2], ah[k][3], b0.x, b1.x);
-                    mma16816(d[1], ah[k][0], ah[k][1], ah[k][2], ah[k][3], b0.y, b1.y);
-                }
-                mma16816(d[0], al[k][0], al[k][1], al[k][2], al[k][3], b0.x, b1.x);
-                mma16816(d[1], al[k][0], al[k][1], al[k][2], al[k][3], b0.y, b1.y);
+                for (int i = 0; i < 4; ++i) { d[i >> 1][i & 1] = s[0][i]; d[i >> 1][2 + (i & 1)] = s[1][i]; }
+            }
+#pragma unroll
+            for (int k = 0; k < 2 * KB; k += 2) {
+                const uint2 p0 = *reinterpret_cast<const uint2*>(pair0 + 4 * k * Sh::PAIR_PITCH + 16 * q);
+                const uint2 p1 = *reinterpret_cast<const uint2*>(pair0 + 4 * (k + 1) * Sh::PAIR_PITCH + 16 * q);
+                const uint32_t b[2][2] = {{p0.x, p0.y}, {p1.x, p1.y}};
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const float2 f = __half22float2(bits_h2(b[half][n]));
+                        mma1688(d[n], ah[k + half], f.x, f.y);
+                        mma1688(d[n], al[k + half], f.x, f.y);
+                    }
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                s[0][i] = fmaf(d[i >> 1][i & 1], p2.down, s[0][i]);
-                s[1][i] = fmaf(d[i >> 1][2 + (i & 1)], p2.down, s[1][i]);
+                s[0][i] = KB == 1 ? d[i >> 1][i & 1] : s[0][i] + d[i >> 1][i & 1];
+                s[1][i] = KB == 1 ? d[i >> 1][2 + (i & 1)] : s[1][i] + d[i >> 1][2 + (i & 1)];
             }
         };
         if constexpr (MODE == 1) {

@@ -508,3 +508,35 @@ def test_arrays_off_by_an_element(ctx, which, bits):
             c.S, c.size, c.err = held, np.abs(held), np.zeros_like(held)
         else:
             assert (np.abs(held - c.S) <= c.tol() + U * np.abs(c.S)).all()
+
+
+class SizedTokens(Cache):
+    """Tokens whose x, or whose B, differ in size by up to 2^30 from row to row, or from token to token."""
+
+    def __init__(self, ctx, d, rng, kind, big):
+        self.kind, self.big, self.made = kind, big, 0
+        super().__init__(ctx, d, rng, np.zeros((d.batch, d.H, d.P, d.N)))
+
+    def token(self, rng):
+        x, Bm, Cm, raw = super().token(rng)
+        if self.kind == "rows":   # one row in eight is `big`, the others are smaller by any factor
+            size = self.big * np.exp(-rng.uniform(0, 20.7, x.shape))
+            size[..., ::8] = self.big
+        else:                     # every other token is `big` and adds nothing: the state is the other tokens'
+            size = self.big if self.made % 2 else 1e-3
+            if self.made % 2:
+                Bm = np.zeros_like(Bm)
+        self.made += 1
+        x = (np.sign(x.astype(np.float64)) * size * rng.uniform(0.5, 1, x.shape)).astype(np.float16)
+        return x, Bm, (Cm.astype(np.float32) * 1e-2).astype(np.float16), raw
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("shape", [(2, 4, 64, 128, 1, 5), (1, 3, 64, 64, 1, 4), (1, 2, 48, 256, 1, 3), (1, 2, 64, 128, 1, 20),
+                                   (2, 3, 75, 203, 1, 16), (1, 2, 20, 260, 2, 3)])
+@pytest.mark.parametrize("kind,big", [("rows", 1000.0), ("rows", 30000.0), ("tokens", 30000.0)])
+def test_rows_and_tokens_of_different_sizes(ctx, shape, bits, kind, big):
+    """A row's digits do not depend on its neighbours', nor a token's on the others': the bounds of every other test."""
+    rng = np.random.default_rng(shape[3] + bits)
+    run_tokens(SizedTokens(ctx, dims(*shape, bits), rng, kind, big), rng, min(2 * shape[5] + 1, 40))
