@@ -787,11 +787,14 @@ cudaError_t launch_tc(const StateCacheArgs& a, cudaStream_t s) {
     uint32_t heads = PAD ? 1 : TC_HEADS;
     while (heads > 1 && (heads * a.P > TC_THREADS || heads * a.P * N * sizeof(Code) > TC_BYTES ||
                          (uint64_t)a.batch * a.G * ((per_group + heads - 1) / heads) < 2ull * 148)) heads /= 2;
-    const uint32_t bytes = TcShared<Code, KB, N>(PAD ? (a.P + 15) / 16 * 16 : heads * a.P).total +
-                           (PAD && MODE == 1 && staged_load(a) ? TC_WARPS * 16 * STAGE_PITCH * 4 : 0);
+    constexpr uint32_t STAGE = PAD && MODE == 1 ? TC_WARPS * 16 * STAGE_PITCH * 4 : 0;
+    const uint32_t bytes = TcShared<Code, KB, N>(PAD ? (a.P + 15) / 16 * 16 : heads * a.P).total + (STAGE && staged_load(a) ? STAGE : 0);
     const auto kernel = k_state_tc<Code, MODE, KB, N, PAD>;
     if (bytes > 36 * 1024) {   // with the static part, more than 48 KB
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        // The limit is the kernel's, for every thread of the process: set to what the largest call takes, so that no
+        // thread's smaller call lowers it between another's set and launch.
+        const int most = (int)(TcShared<Code, KB, N>(TC_THREADS).total + STAGE);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (e != cudaSuccess) return e;
     }
     kernel<<<dim3((per_group + heads - 1) / heads, a.G, a.batch), TC_THREADS, bytes, s>>>(a, heads, per_group);

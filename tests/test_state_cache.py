@@ -540,3 +540,39 @@ def test_rows_and_tokens_of_different_sizes(ctx, shape, bits, kind, big):
     """A row's digits do not depend on its neighbours', nor a token's on the others': the bounds of every other test."""
     rng = np.random.default_rng(shape[3] + bits)
     run_tokens(SizedTokens(ctx, dims(*shape, bits), rng, kind, big), rng, min(2 * shape[5] + 1, 40))
+
+
+@pytest.mark.gpu
+def test_two_threads_with_different_shapes(ctx):
+    """A context a host thread, over shapes whose launches want different amounts of shared memory: no call of one is
+    refused for the other's."""
+    import threading
+
+    failed, start = [], threading.Barrier(2)
+
+    def work(P):
+        try:
+            c = lssm.Ctx(0)
+            d = dims(1, 1, P, 255, 1, 20, 16)
+            cache, ops = lssm.StateCache(c, d), lssm.Ops(c)
+            A = lssm.DeviceBuffer.from_array(c, np.zeros(1, np.float16))
+            out = lssm.DeviceBuffer(c, P * 255 * 2)
+            start.wait()
+            for _ in range(20):
+                c.begin_batch()
+                try:
+                    for _ in range(300):
+                        ops.state_cache_load(cache, A, out, lssm.DT_F16, d)
+                finally:
+                    c.commit_and_wait()
+            c.close()
+        except Exception as e:   # noqa: BLE001
+            failed.append((P, repr(e)))
+            start.abort()
+
+    threads = [threading.Thread(target=work, args=(P,)) for P in (150, 255)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
