@@ -35,6 +35,7 @@ lssm_status fail(lssm_status st, const char* fmt, ...) {
 }
 
 lssm_status cuda_fail(cudaError_t e, const char* what) {
+    cudaGetLastError();   // reported here: the thread's next call does not find it again
     if (e == cudaErrorMemoryAllocation)
         return fail(LSSM_ERR_OUT_OF_MEMORY, "%s: %s", what, cudaGetErrorString(e));
     if (e == cudaErrorInvalidValue)

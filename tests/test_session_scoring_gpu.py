@@ -321,3 +321,22 @@ def test_score_and_cached_decode_together(ctx, bits):
     assert worst <= tol
     a.close()
     b.close()
+
+
+def test_a_failed_decode_does_not_fail_the_next_call(ctx):
+    """The error of a step that cannot be captured (the default stream) is reported once."""
+    c = lssm.Ctx(0)
+    c.set_stream(0)
+    hp, m = make(c, seed=16)
+    tok = np.random.default_rng(2).integers(0, 1000, (3, 6)).astype(np.uint32)
+    s = lssm.Session(c, m, batch=3, max_seq_len=6)
+    first = s.prefill(tok)
+    with pytest.raises(lssm.LssmError, match="captur"):
+        s.decode(first, 2)
+    s.set_option("cuda_graph", 0)
+    q = lssm.Session(c, m, batch=3, max_seq_len=6)
+    q.set_option("cuda_graph", 0)
+    assert np.array_equal(s.decode(first, 2), q.decode(q.prefill(tok), 2))
+    s.close()
+    q.close()
+    c.close()
