@@ -1019,13 +1019,15 @@ static StateCacheArgs cache_args(const lssm_session* s, uint32_t layer) {
     a.dt_min = 1e-6f; a.dt_max = 1e6f; a.has_D = 1;
     return a;
 }
-// The states from where they are to the other place: into the cache (`in_cache` is set by the caller, before it
-// captures a step over it) or back to fp32.
+// The states from where they are to the other place, into the cache or back to fp32. `in_cache` changes when all
+// layers' launches are made: a call that ends before leaves the states where they were.
 static lssm_status states_to_cache(lssm_session* s, cudaStream_t st) {
+    if (s->in_cache) return LSSM_OK;
     for (uint32_t l = 0; l < s->m->img.hdr.n_layer; ++l) {
         CU(launch_state_store(cache_args(s, l), st));
         s->nl += 1;
     }
+    s->in_cache = true;
     return LSSM_OK;
 }
 static lssm_status states_to_f32(lssm_session* s, cudaStream_t st) {
@@ -1170,7 +1172,7 @@ static lssm_status run_block(lssm_session* s, uint32_t layer, uint32_t L, bool d
         a.batch = B; a.H = H; a.P = P; a.N = N; a.G = s->G;
         a.dt_min = 1e-6f; a.dt_max = 1e6f; a.has_D = 1;
         a.x_bs = di; a.bc_bs = GN; a.dt_bs = proj; a.y_bs = di; a.z_bs = proj;
-        if (s->in_cache) {
+        if (s->state_bits) {   // over the cache, where lssm_decode puts the states before the first step runs
             StateCacheArgs c = cache_args(s, layer);
             c.x = a.x; c.B = a.B; c.C = a.C; c.dt_raw = a.dt_raw; c.dt_bias = a.dt_bias; c.D = a.D;
             c.y = a.y; c.z = a.z;
@@ -1480,8 +1482,6 @@ extern "C" lssm_status lssm_decode(lssm_session* s, const uint32_t* first, uint3
         return check_err(s, "decode");
     }
     CU(launch_embed_gather(s->d_cur, W(m, m->embed), s->hidden, s->batch, h.d_model, h.vocab_size, s->d_err, st));
-    const bool quantise = s->state_bits && !s->in_cache;
-    s->in_cache = s->state_bits != 0;
     if (s->use_graph && !s->graph) {
         cudaGraph_t g;
         CU(cudaStreamBeginCapture(st, cudaStreamCaptureModeThreadLocal));
@@ -1489,20 +1489,15 @@ extern "C" lssm_status lssm_decode(lssm_session* s, const uint32_t* first, uint3
         lssm_status r = decode_step_body(s, st);
         s->decode_step_launches = s->nl - nl0;
         cudaError_t e = cudaStreamEndCapture(st, &g);
-        if (r || e != cudaSuccess) s->in_cache = s->in_cache && !quantise;
         if (r) { if (e == cudaSuccess) cudaGraphDestroy(g); return r; }
         if (e != cudaSuccess) return cuda_fail(e, "decode graph capture");
         e = cudaGraphInstantiate(&s->graph, g, 0);
         cudaGraphDestroy(g);
-        if (e != cudaSuccess) {
-            s->graph = nullptr;
-            s->in_cache = s->in_cache && !quantise;
-            return cuda_fail(e, "decode graph instantiate");
-        }
+        if (e != cudaSuccess) { s->graph = nullptr; return cuda_fail(e, "decode graph instantiate"); }
     }
     CU(cudaEventRecord(s->ev[2], st));
-    if (quantise)
-        if (lssm_status r = states_to_cache(s, st)) { s->in_cache = false; return r; }
+    if (s->state_bits)
+        if (lssm_status r = states_to_cache(s, st)) return r;
     for (uint32_t i = 0; i < n_steps; ++i) {
         if (s->graph) CU(cudaGraphLaunch(s->graph, st));
         else {

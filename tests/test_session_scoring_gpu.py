@@ -340,3 +340,34 @@ def test_a_failed_decode_does_not_fail_the_next_call(ctx):
     s.close()
     q.close()
     c.close()
+
+
+def test_failed_decode_leaves_the_states_where_they_were(ctx):
+    """A decode that ends before the states are quantised (a step cannot be captured on the default stream): later calls
+    go on from the states of the prefill."""
+    c = lssm.Ctx(0)
+    c.set_stream(0)
+    hp, m = make(c, seed=17)
+    rng = np.random.default_rng(3)
+    prompt, seq = rng.integers(0, 1000, (3, 20)).astype(np.uint32), rng.integers(0, 1000, (3, 8)).astype(np.uint32)
+
+    def session(fail):
+        s = lssm.Session(c, m, batch=3, max_seq_len=20)
+        s.set_option("state_bits", 8)
+        s.prefill(prompt)
+        if fail:
+            with pytest.raises(lssm.LssmError):
+                s.decode(seq[:, 0], 1)
+        s.set_option("cuda_graph", 0)
+        return s
+
+    goes_on = [lambda s: forced(s, seq, 8, 0),                                  # a decode over the cache
+               lambda s: (s.prefill(seq), s.logits())[1],                       # a prefill, from fp32 states
+               lambda s: (s.set_option("state_bits", 16), forced(s, seq, 8, 0))[1],
+               lambda s: s.score(seq)[0]]
+    for go in goes_on:
+        a, b = session(False), session(True)
+        assert np.array_equal(go(b), go(a))
+        a.close()
+        b.close()
+    c.close()
