@@ -384,7 +384,8 @@ lssm_status lssm_session_logits(lssm_session* s, float* out);
  * top_ids / top_logp batch x L x top_k) is lssm_logprobs of the logits after token i with token i + 1 as
  * the target; the last entry's logp is 0 (no target). -mean(logp[:-1]) is the mean negative log
  * likelihood, its exponential the perplexity. Any output may be null, but not all. Afterwards the session
- * is where lssm_prefill of the same tokens leaves it. Not for tensor-parallel sessions (LSSM_ERR_STATE). */
+ * is where lssm_prefill of the same tokens leaves it, and the last entries are what lssm_session_logprobs
+ * gives there. Not for tensor-parallel sessions (LSSM_ERR_STATE). */
 lssm_status lssm_score(lssm_session* s, const uint32_t* tokens, uint32_t L, uint32_t top_k, float* logp,
                        float* entropy, uint32_t* top_ids, float* top_logp);
 /* lssm_logprobs of the logits of the last position computed, one row per sequence (host arrays of batch,

@@ -1312,7 +1312,8 @@ extern "C" lssm_status lssm_prefill(lssm_session* s, const uint32_t* tokens, uin
 }
 
 // ---- scoring ---------------------------------------------------------------------
-// Device block of the scoring calls: logits of `run` rows, then targets and results of `rows` rows.
+// Device block of the scoring calls: logits of `run` rows, then targets and results of `rows` rows (a score's last
+// positions twice).
 struct ScoreBlock {
     __half* logits;
     uint32_t *targets, *ids;
@@ -1385,11 +1386,11 @@ extern "C" lssm_status lssm_score(lssm_session* s, const uint32_t* tokens, uint3
     // the vocabulary's logits of a run of rows at a time: 64 MiB, at least a tile of the GEMM
     const size_t run = std::min(rows, std::max<size_t>(128, ((size_t)64 << 20) / ((size_t)s->V * 2) / 128 * 128));
     ScoreBlock b;
-    if (lssm_status r = score_block(s, rows, run, top_k, &b)) return r;
+    if (lssm_status r = score_block(s, rows + s->batch, run, top_k, &b)) return r;
     const uint64_t nl0 = s->nl;
     if (lssm_status r = forward_rows(s, tokens, L, st)) return r;
     // row i's target is token i + 1 of its sequence; the last row has none
-    CU(cudaMemsetAsync(b.targets, 0xFF, rows * 4, st));
+    CU(cudaMemsetAsync(b.targets, 0xFF, (rows + s->batch) * 4, st));
     if (L > 1)
         CU(cudaMemcpy2DAsync(b.targets, (size_t)L * 4, s->d_tokens + 1, (size_t)L * 4, (size_t)(L - 1) * 4, s->batch,
                              cudaMemcpyDeviceToDevice, st));
@@ -1400,6 +1401,18 @@ extern "C" lssm_status lssm_score(lssm_session* s, const uint32_t* tokens, uint3
         if (lssm_status r = score_rows(s, b.logits, b, r0, n, top_k, st)) return r;
     }
     if (lssm_status r = pick_tokens(s, s->lastrows, false, st)) return r;
+    // a sequence's last entry is of the logits that the session holds from here on: another kernel's than its run's
+    // where the runs have more than 8 rows, so a last bit may differ
+    if (lssm_status r = score_rows(s, s->logits, b, rows, s->batch, top_k, st)) return r;
+    auto to_last = [&](void* all, size_t each) {
+        uint8_t* p = static_cast<uint8_t*>(all);
+        return cudaMemcpy2DAsync(p + (L - 1) * each, L * each, p + rows * each, each, each, s->batch, cudaMemcpyDeviceToDevice, st);
+    };
+    CU(to_last(b.entropy, 4));
+    if (top_k) {
+        CU(to_last(b.ids, (size_t)top_k * 4));
+        CU(to_last(b.top, (size_t)top_k * 4));
+    }
     s->prefill_launches = s->nl - nl0;
     CU(cudaEventRecord(s->ev[1], st));
     if (lssm_status r = score_results(b, rows, top_k, logp, entropy, top_ids, top_logp, st)) return r;

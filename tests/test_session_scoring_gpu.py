@@ -371,3 +371,19 @@ def test_failed_decode_leaves_the_states_where_they_were(ctx):
         a.close()
         b.close()
     c.close()
+
+
+@pytest.mark.parametrize("batch,L", [(1, 1), (1, 40), (3, 33), (12, 5)])
+def test_score_ends_with_the_logits_it_leaves(ctx, batch, L):
+    """The last entry of every sequence is of the very logits that the session holds afterwards, and that the greedy
+    pick was made of."""
+    hp, m = make(ctx, seed=11)
+    tok = np.random.default_rng(batch).integers(0, 1000, (batch, L)).astype(np.uint32)
+    s = lssm.Session(ctx, m, batch=batch, max_seq_len=L)
+    logp, ent, ids, top = s.score(tok, 6)
+    _, e, i, t = s.logprobs(np.full(batch, lssm.NO_TOKEN, np.uint32), 6)
+    assert np.array_equal(ent[:, -1], e) and np.array_equal(ids[:, -1], i) and np.array_equal(top[:, -1], t)
+    assert np.array_equal(ids[:, -1, 0], s.logits().argmax(1)) and (logp[:, -1] == 0).all()
+    only = s.score(tok)[1]   # a continuation: other numbers, the same rule, without alternatives
+    assert np.array_equal(only[:, -1], s.logprobs(np.zeros(batch))[1])
+    s.close()
