@@ -266,8 +266,8 @@ lssm_status lssm_logprobs(lssm_ctx* ctx, const void* logits, const uint32_t* tar
  *   dlogits_j = g_logp ([j = t] - p_j) - g_entropy p_j (log p_j + entropy)
  * lse and entropy (rows) are lssm_logprobs' outputs for the same logits; g_logp / g_entropy (rows)
  * are the gradients of a scalar with respect to those outputs, null = none (not both); g_logp needs
- * targets, g_entropy needs entropy. A LSSM_NO_TOKEN row takes nothing from g_logp, a row with lse -inf
- * is 0, an id >= vocab makes the row NaN. lse, the alternatives and their order carry no gradient.
+ * targets, g_entropy needs entropy. A LSSM_NO_TOKEN row takes nothing from g_logp, an id >= vocab
+ * makes the row NaN, any other row with lse -inf is 0. lse, the alternatives and their order carry no gradient.
  * dlogits is of grad_dtype, grad_stride elements apart (0 = vocab); it may be the logits themselves
  * (same address, type and stride), and must not overlap them otherwise. */
 typedef struct {

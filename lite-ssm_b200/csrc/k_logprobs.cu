@@ -616,15 +616,16 @@ struct GradRow {
         t = a.targets ? a.targets[r] : LSSM_NO_TOKEN;
         h = a.g_entropy ? a.g_entropy[r] : 0.0f;
         H = a.g_entropy ? a.entropy[r] : 0.0f;
-        none = lse == -INFINITY;
+        const bool outside = t != LSSM_NO_TOKEN && t >= a.vocab;
+        none = lse == -INFINITY && !outside;
         g = a.g_logp && t != LSSM_NO_TOKEN ? a.g_logp[r] : 0.0f;
-        if (t != LSSM_NO_TOKEN && t >= a.vocab) g = __int_as_float(0x7FC00000);
+        if (outside) g = __int_as_float(0x7FC00000);
     }
     template <bool ENTROPY>
     __device__ __forceinline__ float operator()(float x, uint32_t j) const {
         const float lp = x - lse, p = ex2(lp * LOG2E);
-        // p = 0 ends a masked entry: its log p may be -inf
-        const float d = ENTROPY ? (p == 0.0f ? 0.0f : -p * fmaf(h, lp + H, g)) : -p * g;
+        // p = 0 ends a masked entry, whose log p may be -inf: what is left is -p g, 0, or NaN for a target outside
+        const float d = ENTROPY && p != 0.0f ? -p * fmaf(h, lp + H, g) : -p * g;
         return none ? 0.0f : j == t ? d + g : d;
     }
 };

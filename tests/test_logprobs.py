@@ -477,3 +477,26 @@ def test_logprobs_two_contexts_on_streams_of_their_own(ctx):
         check_rows(got, x64, t, V, k)
     for c in cs:
         c.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_logprobs_backward_target_outside_the_vocabulary(ctx, dt):
+    """Such a row is NaN throughout: masked entries, entries whose p is 0 and rows that a mask leaves empty among them,
+    with either gradient or both. Rows beside it are not touched by it."""
+    V = 203
+    rng = np.random.default_rng(7)
+    x = logits(rng, 6, V)
+    x[1, ::3] = -np.inf
+    x[2] = -np.inf
+    x[3, 1:] -= 2000.0
+    arr, x64 = encode(x, dt)
+    t = np.array([V, V + 1, V, NONE - 1, 3, NONE], np.uint32)
+    tr = [truth(r, NONE, 0) for r in x64]
+    lse, ent = [a[0] for a in tr], [a[2] for a in tr]
+    g, h = np.full(6, 1.5, np.float32), np.full(6, -0.5, np.float32)
+    for gg, hh in ((g, None), (g, h), (None, h)):
+        got = backward(ctx, arr, t, lse, ent, gg, hh, V, dt, lssm.DT_F32)
+        assert np.isnan(got[:4]).all()
+        check_grad(got[4:], x64[4:], t[4:] if gg is not None else np.full(2, NONE, np.uint32), (gg if gg is not None else 0 * g)[4:],
+                   (hh if hh is not None else 0 * h)[4:], lssm.DT_F32)
