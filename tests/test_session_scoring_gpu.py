@@ -387,3 +387,42 @@ def test_score_ends_with_the_logits_it_leaves(ctx, batch, L):
     only = s.score(tok)[1]   # a continuation: other numbers, the same rule, without alternatives
     assert np.array_equal(only[:, -1], s.logprobs(np.zeros(batch))[1])
     s.close()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_cached_decode_of_a_tensor_parallel_session(ctx, bits):
+    """A communicator of one rank: the sharded path over the cache, against its own fp32 states until the first fold and,
+    with 16 bits, behind it, and back to fp32 before a prefill and by the option; with 8 bits, in one call or in several."""
+    hp, m = make(ctx, seed=19, n_groups=2)
+    rng = np.random.default_rng(5)
+    prompt, seq, more = (rng.integers(0, 1000, (3, n)).astype(np.uint32) for n in (16, 30, 9))
+    comm = lssm.Comm(ctx, 0, 1, bytes(lssm.COMM_ID_BYTES))
+    a, b = (lssm.Session(ctx, m, batch=3, max_seq_len=16, comm=comm) for _ in range(2))
+    b.set_option("state_bits", bits)
+    b.set_option("state_window", 7)
+    close_logits(forced(b, seq, 6, 0), forced(a, seq, 6, 0))   # from zero: nothing is rounded before the fold
+    for s in (a, b):
+        s.reset()
+        s.prefill(prompt)
+    if bits == 16:
+        close_logits(forced(b, seq, 25, 0), forced(a, seq, 25, 0))
+        for s in (a, b):
+            s.prefill(more)
+        close_logits(forced(b, seq, 3, 25), forced(a, seq, 3, 25))
+        b.set_option("state_bits", 0)
+        close_logits(forced(b, seq, 3, 0), forced(a, seq, 3, 0))
+    else:   # folds at different places of a call, captured or not
+        one = lssm.Session(ctx, m, batch=3, max_seq_len=16, comm=comm)
+        one.set_option("state_bits", 8)
+        one.set_option("state_window", 7)
+        one.set_option("cuda_graph", 0)
+        cur = one.prefill(prompt)
+        for s in (one, b):
+            s.reset()
+            s.prefill(prompt)
+        first, second = b.decode(cur, 9), one.decode(cur, 20)
+        assert np.array_equal(np.concatenate([first, b.decode(first[:, -1], 11)], 1), second)
+        assert np.array_equal(b.logits(), one.logits())
+        one.close()
+    a.close()
+    b.close()
