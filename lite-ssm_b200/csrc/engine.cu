@@ -1053,9 +1053,7 @@ static lssm_status set_state_cache(lssm_session* s, uint32_t bits, uint32_t wind
     if (!layer) return fail(LSSM_ERR_INVALID_ARGUMENT, "lssm_session_set_option: the model's shape has no state cache");
     if (lssm_status r = s_alloc(reinterpret_cast<void**>(&s->d_cache), layer * s->m->img.hdr.n_layer, "session: state cache"))
         return r;
-    // windows are read up to their fill only; the rest stays zero
-    CU(cudaMemsetAsync(s->d_cache, 0, layer * s->m->img.hdr.n_layer, s->ctx->stream));
-    s->state_bits = bits;
+    s->state_bits = bits;   // the store of the next decode writes codes, scales and fill; windows are read up to their fill
     return LSSM_OK;
 }
 

@@ -426,3 +426,27 @@ def test_cached_decode_of_a_tensor_parallel_session(ctx, bits):
         one.close()
     a.close()
     b.close()
+
+
+def test_cached_decode_on_another_stream_than_the_option(ctx):
+    """Setting state_bits leaves nothing under way on the context's stream that a decode on the next one could meet."""
+    import torch
+
+    c = lssm.Ctx(0)
+    hp, m = make(c, seed=23)
+    rng = np.random.default_rng(1)
+    prompt, seq = rng.integers(0, 1000, (48, 6)).astype(np.uint32), rng.integers(0, 1000, (48, 4)).astype(np.uint32)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for switch in (False, True, True):
+        c.set_stream(streams[0].cuda_stream)
+        s = lssm.Session(c, m, batch=48, max_seq_len=6)
+        s.set_option("cuda_graph", 0)
+        s.prefill(prompt)
+        s.set_option("state_bits", 16)
+        if switch:
+            c.set_stream(streams[1].cuda_stream)
+        outs.append(forced(s, seq, 4, 0))
+        s.close()
+    assert np.array_equal(outs[1], outs[0]) and np.array_equal(outs[2], outs[0])
+    c.close()
