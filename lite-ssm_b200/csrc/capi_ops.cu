@@ -712,6 +712,7 @@ lssm_status lssm_state_cache_load(lssm_ctx* ctx, lssm_state_cache cache, const v
     a.A_log = static_cast<const __half*>(A_log);
     a.state = state; a.state_dtype = state_dtype;
     CHECK_CTX(ctx);
+    a.sm_count = ctx->sm_count;
     LAUNCH("state_cache_load", launch_state_load(a, ctx->stream));
 }
 
@@ -736,6 +737,7 @@ lssm_status lssm_ssd_step_cached(lssm_ctx* ctx, const void* x, const void* B, co
     a.y = static_cast<__half*>(y);
     a.x_bs = (uint64_t)d.H * d.P; a.bc_bs = (uint64_t)a.G * d.N; a.dt_bs = d.H; a.y_bs = a.x_bs;
     CHECK_CTX(ctx);
+    a.sm_count = ctx->sm_count;
     LAUNCH("ssd_step_cached", launch_ssd_step_cached(a, ctx->stream));
 }
 

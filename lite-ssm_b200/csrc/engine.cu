@@ -1017,6 +1017,7 @@ static StateCacheArgs cache_args(const lssm_session* s, uint32_t layer) {
     a.batch = s->batch; a.H = s->H; a.P = h.d_head; a.N = h.d_state; a.G = s->G;
     a.W = s->state_window; a.bits = s->state_bits;
     a.dt_min = 1e-6f; a.dt_max = 1e6f; a.has_D = 1;
+    a.sm_count = s->ctx->sm_count;
     return a;
 }
 // The states from where they are to the other place, into the cache or back to fp32. `in_cache` changes when all

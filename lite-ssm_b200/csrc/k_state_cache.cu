@@ -782,11 +782,15 @@ __global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateC
 template <typename Code, int MODE, int KB, int N, bool PAD>
 cudaError_t launch_tc(const StateCacheArgs& a, cudaStream_t s) {
     // Heads of a group share the window's B and what is computed from it: as many as TC_BYTES of codes allow, fewer
-    // where the grid would leave SMs without a CTA.
+    // where less than two CTAs an SM would be left. Steps without folds, with 1 / 2 / 4 heads a CTA of 64 x 128, W 16: 8 bits,
+    // 80 heads, 64 sequences 28.9 / 20.1 / 17.1 us, 16 10.6 / 9.8 / 8.2, 2 4.5 / 4.9 / 6.1; all folding, 8 sequences 17.9 /
+    // 14.4 / 17.3, 2 8.4 / 9.8 / 12.4. 16 bits (64 KB of codes for four), 64 sequences 32.9 / 25.5 / 27.7, all folding
+    // 91.9 / 76.9 / 82.3. (One sequence in 16 folding, 64 sequences of 8 bits: 33.5 / 25.9 / 27.7, but the host does not
+    // know which do, and a session's sequences fold together.)
     const uint32_t per_group = a.H / a.G;
     uint32_t heads = PAD ? 1 : TC_HEADS;
     while (heads > 1 && (heads * a.P > TC_THREADS || heads * a.P * N * sizeof(Code) > TC_BYTES ||
-                         (uint64_t)a.batch * a.G * ((per_group + heads - 1) / heads) < 2ull * 148)) heads /= 2;
+                         (uint64_t)a.batch * a.G * ((per_group + heads - 1) / heads) < 2ull * (uint32_t)a.sm_count)) heads /= 2;
     constexpr uint32_t STAGE = PAD && MODE == 1 ? TC_WARPS * 16 * STAGE_PITCH * 4 : 0;
     const uint32_t bytes = TcShared<Code, KB, N>(PAD ? (a.P + 15) / 16 * 16 : heads * a.P).total + (STAGE && staged_load(a) ? STAGE : 0);
     const auto kernel = k_state_tc<Code, MODE, KB, N, PAD>;

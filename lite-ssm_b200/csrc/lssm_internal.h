@@ -171,6 +171,7 @@ struct StateCacheArgs {
     float dt_min, dt_max;
     uint32_t has_D;
     uint64_t x_bs, bc_bs, dt_bs, y_bs, z_bs;
+    int sm_count;
 };
 cudaError_t launch_state_store(const StateCacheArgs& a, cudaStream_t s);
 cudaError_t launch_state_load(const StateCacheArgs& a, cudaStream_t s);
