@@ -292,7 +292,8 @@ lssm_status lssm_logprobs_backward(lssm_ctx* ctx, const void* logits, const uint
  *   fill    (batch, H) u32                    tokens in the window, 0 .. window - 1; a sequence's heads alike
  * A step whose token fills the window folds it into the codes (the state is rounded once in `window`
  * tokens, to the nearest code, ties to even) and empties it. A row of N that holds a NaN or an
- * infinity reads back as NaN; a row with max < 1.2e-38 * Q (Q = 127 or 32767) as 0.
+ * infinity reads back as NaN; a row with max < 1.2e-38 * Q (Q = 127 or 32767) as 0. What a token of the
+ * window makes infinite reads back as infinite or NaN.
  * All arrays are batch-major, so a range of sequences is the arrays from its first sequence on.
  * N 64, 128 or 256 with P a multiple of 16 and 16-byte aligned arrays is read in whole pieces; every
  * other shape and alignment works, slower.

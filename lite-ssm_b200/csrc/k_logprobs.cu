@@ -444,9 +444,9 @@ __device__ __forceinline__ void cta_top(const Row<T>& row, uint32_t c0, uint32_t
 // goes through memory, so there is no workspace and no second launch.
 //
 // Why so: 256 threads x 2 groups of 4 x 16 bytes on their way, 4 CTAs an SM, put 128 KB of loads on an SM; the
-// registers (64 a thread) allow no more. fp16 entries are worked on two a time (f32x2), with one ex2 each.
-// What bounds it, at 2048 x 50288 fp16 with 20 alternatives: 47.1 us = 4.4 TB/s, 67 % of a copy's rate. Without
-// alternatives 41 us, as a pass that only reads in this loop takes 37: the selection after a CTA's pass (barriers and
+// registers (64 a thread, and 16 bytes a thread spilled with fp16) allow no more. fp16 entries are worked on two a time (f32x2), with one ex2 each.
+// What bounds it, at 2048 x 50288 fp16 with 20 alternatives: 47.1-49.1 us = 4.2-4.4 TB/s, 64-67 % of a copy's rate.
+// Without alternatives 38.4 us, as a pass that only reads in this loop takes 37: the selection after a CTA's pass (barriers and
 // second reads, a third of its cycles) leaves HBM idle where the other CTAs of the SM are in it too, and 2048 rows are
 // 3.5 waves. 333 x 32001 fp32, 8 alternatives: 14.4 us; 64 x 256000 fp16, 5 of them: 14.4 us; one row of 50288: 8.2 us,
 // latency of a launch, of reads one after the other and of barriers.
@@ -512,7 +512,9 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) k_logprobs(LogprobsArgs a
         work(next);
     }
     // HBM has nothing to do for this CTA from here on: the beginning of the row one full GPU of CTAs ahead goes to L2
-    // (2048 x 50288 fp16, 20 alternatives: 50.4 us without, 49.2 with 16 KB, 47.1 with 32 or 64, 51.1 with 128).
+    // (2048 x 50288 fp16, 20 alternatives: 50.5 us without, 49.3 with 16 KB, 47.2 with 32, 47.7 with 64, 51.1 with 128;
+    // none 41.1, 39.7, 38.4, 39.3; 2048 x 32001 fp32 55.3, 53.4, 52.4, 51.9; 1024 x 100000 47.2, 47.2, 47.4, 49.3; 4096 x
+    // 32000 63.3, 61.6, 61.5, 61.5; rows of 256000, and no more rows than CTAs: the same with and without).
     const uint64_t later = (uint64_t)r + (uint32_t)(a.sm_count * LP_CTAS);
     if (nc == 1 && tid == 0 && later < a.rows) {
         const Row<T> next_row(a.logits, later * a.row_stride, a.vocab);
@@ -658,7 +660,7 @@ __device__ __forceinline__ void store_chunk(G* p, const float (&v)[n]) {
 // logits); all of them are loaded before the first is worked on. Where the chunks' places in the output are not
 // aligned for wide stores, a warp exchanges its 32 chunks through shared memory, so that a store instruction
 // writes 32 neighbours.
-// Bound by HBM: 2048 x 50288 fp16 to fp16 69.6 us = 5.9 TB/s, 90 % of a copy's rate (the same with a third fewer
+// Bound by HBM: 2048 x 50288 fp16 to fp16 69.6-73.1 us = 5.6-5.9 TB/s, 86-90 % of a copy's rate (the same with a third fewer
 // instructions, in pairs of entries: not kept); 257 x 32001 bf16 to fp32 with the entropy's term, rows at odd addresses,
 // 12.6 us = 3.9 TB/s (35 us with stores of one element, before the exchange), where a launch's ends weigh more.
 constexpr int GRAD_CHUNKS = 4;

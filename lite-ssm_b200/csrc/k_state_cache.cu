@@ -394,7 +394,7 @@ __host__ __device__ __forceinline__ bool staged_load(const StateCacheArgs& a) { 
 // (ssd_step_batched) takes 51 us each time. 16 bits: 25.0 us. One sequence of 24 heads: 4.1 us, a launch's latency.
 // A load of the same 64 sequences takes 31.1 us to fp16 (126 MB, 4.1 TB/s; shared memory's and the products' latency)
 // and 38.8 us to fp32 (210 MB, 5.4 TB/s; HBM).
-// 16 sequences x 64 heads of 75 x 203, 8 bits, padded: 28 us a step (55 on the CUDA cores).
+// 16 sequences x 64 heads of 75 x 203, 8 bits, padded: 29 us a step (55 on the CUDA cores).
 // Measured and not kept: a persistent CTA with the next heads' codes on their way (24.8-30 us against 23.8 at the time:
 // registers for two of everything leave 2 CTAs an SM), codes in two parts that are waited for one after the other
 // (18.6 against 17.2), all W rows of the window read without waiting for `fill` (19.3; one sequence 5.0 against 4.1),
@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(TC_THREADS, KB == 1 ? 4 : 3) k_state_tc(StateC
                 }
             } else if (PAD && staged_load(a)) {
                 // 16 rows x 32 columns at a time through shared memory, so that a store instruction writes 32 neighbours
-                // (16 x 64 heads of 75 x 203, 8 bits, to fp16: 59 -> 43 us; to fp32, whose stores of one element fill
+                // (16 x 64 heads of 75 x 203, 8 bits, to fp16: 59 -> 43 us when it came, 45 now; to fp32, whose stores of one element fill
                 // more of a line, it costs 5 %)
                 float(*stage)[STAGE_PITCH] = reinterpret_cast<float(*)[STAGE_PITCH]>(sm + sh.total) + 16 * wid;
                 const uint64_t t0 = ((uint64_t)bh0 * a.P + tile * 16) * n_real;
