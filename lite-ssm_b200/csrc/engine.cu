@@ -1456,6 +1456,7 @@ extern "C" lssm_status lssm_decode(lssm_session* s, const uint32_t* first, uint3
     if (n_steps > s->hist_cap) {
         if (s->d_hist) cudaFree(s->d_hist);
         s->d_hist = nullptr;
+        s->hist_cap = 0;   // until the memory is there
         if (s->graph) { cudaGraphExecDestroy(s->graph); s->graph = nullptr; }
         CU(cudaMalloc(&s->d_hist, (size_t)s->batch * n_steps * 4));
         s->hist_cap = n_steps;

@@ -450,3 +450,19 @@ def test_cached_decode_on_another_stream_than_the_option(ctx):
         s.close()
     assert np.array_equal(outs[1], outs[0]) and np.array_equal(outs[2], outs[0])
     c.close()
+
+
+def test_decode_after_a_history_that_did_not_fit(ctx):
+    """A decode of more steps than device memory holds the tokens of is refused, and the next one runs."""
+    hp, m = make(ctx, seed=29)
+    tok = np.random.default_rng(6).integers(0, 1000, (16, 5)).astype(np.uint32)
+    s, q = (lssm.Session(ctx, m, batch=16, max_seq_len=5) for _ in range(2))
+    first = s.prefill(tok)
+    s.decode(first, 2)
+    st = lssm.lib().lssm_decode(s.h, first.ctypes.data_as(lssm.P), 0xFFFFFFFF, None)   # 16 * 2^32 * 4 bytes: 256 GiB
+    assert st != 0
+    cur = q.prefill(tok)
+    q.decode(cur, 2)
+    assert np.array_equal(s.decode(first, 2), q.decode(cur, 2))
+    s.close()
+    q.close()
